@@ -192,9 +192,10 @@ def prepare(case, seed):
                 s["k"], s["v"] = _buf(d["k"]), _buf(d["v"])
             else:  # what earlier steps have written
                 whole = KvSeqs(case["n"], d["ldt"], table, lens, _buf(d["krows_t"]))
+                k, v = _buf(d["k"]), _buf(d["v"])
                 torch.cuda.synchronize()
-                s["cache"].write_bufs(0, whole, sum(d["lens"]), _buf(d["k"]), _buf(d["v"]))
-                _eng().sync()
+                s["cache"].write_bufs(0, whole, sum(d["lens"]), k, v)
+                _eng().sync()  # the rows' buffers go with this call
             if kind == "decode":
                 s["q"] = _buf(d["q"])
         if kind in ("write", "read"):
