@@ -1,0 +1,563 @@
+// Attention of a batch's newest tokens over the paged cache (layouts and the division of work in attn.h).
+//
+// With s_mj = scale q_m . k_j for the keys j that row m sees, o_m = sum_j e^(s_mj - M_m) v_j / sum_j e^(s_mj - M_m): one pass
+// over the pages with the running maximum M and sum L of each row, in f32 and base 2 (the scale carries log2 e). Bound by
+// HBM: every key and value is read once, for all query heads of its key head (and all drafts of its sequence) together.
+//
+// A wave takes a page of 64 keys at a time: S^T = K Q^T on v_mfma_f32_16x16x32 (A: 16 keys, straight from the page's
+// granules; B: 16 query rows, from LDS), the softmax in registers (a lane holds one row's keys; quads share rows, so a
+// maximum is two lane swaps), O^T += V^T P^T (A: 16 dims; B: the weights, which the page's value order leaves in the right
+// lanes). Rows and weights are f32 cut into NS parts of 8 or 11 bits (bf16: three, fp16: two), so that the products carry
+// the f32 operand whole; keys and values are what the cache holds, exactly. The matrix cores have the room: 16 x 32
+// elements take 16 cycles of one SIMD, HBM brings a CU 6.5 bf16 elements a cycle.
+//
+// fp16 parts have fp16's range: a query row is scaled by the power of two that brings its largest element under 1 (taken
+// back in the scores), weights are 2^14 times themselves (so are the sums L), and the steps of 8-bit values, which are
+// weights' factors, are taken relative to the largest power of two that the wave has met (taken back at the end). What a
+// part then drops is 2^-24 of the largest element or weight at most.
+//
+// Work is dealt out in equal shares of pages over one workgroup per CU, so a single long sequence and a ragged batch fill
+// the chip alike; a workgroup's waves take a segment's pages in turn and are joined through LDS, shares of one group
+// through its partials, by the last of them to arrive (a counter; partials are device-coherent stores, so no cache is
+// written back or invalidated).
+#include "attn_device.h"
+#include "common.h"
+
+namespace ijah {
+
+namespace {
+
+constexpr float kNegInf = -__builtin_inff();
+
+// waves of a workgroup: with 256 dims a wave's keys, values and sums take more than the 256 registers of eight waves
+template <int D>
+constexpr int kWaves = D == 256 ? 4 : 8;
+
+template <int KIND>
+struct Num {  // the matrix type of a cache kind, and the parts an f32 operand is cut into
+  static constexpr int NS = KIND == kKvBf16 ? 3 : 2;
+};
+
+template <int KIND>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (KIND == kKvBf16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// the parts of 1, and whether one of a register's two values is not finite (its exponent all ones)
+template <int KIND>
+constexpr uint32_t kOne = KIND == kKvBf16 ? 0x3F80u : 0x3C00u;
+template <int KIND>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {  // all ones in the halves that are not
+  constexpr uint32_t e = KIND == kKvBf16 ? 0x7F80u : 0x7C00u;
+  return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
+}
+__device__ __forceinline__ int again(int v) {  // v as a value of its own from here on: computed here, not held
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// x = part + rest exactly (the subtraction of a value's own rounding is exact)
+template <int KIND>
+__device__ __forceinline__ u32x4 part_of(f32x8 &x) {
+  const u32x4 w = KIND == kKvBf16 ? to_bf16x8(x) : to_f16x8(x);
+  if constexpr (KIND == kKvBf16) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      x[2 * k] -= __uint_as_float(w[k] << 16);
+      x[2 * k + 1] -= __uint_as_float(w[k] & 0xFFFF0000u);
+    }
+  } else {
+    const f16x8 h = __builtin_bit_cast(f16x8, w);
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] -= (float)h[k];
+  }
+  return w;
+}
+
+// the batch's place where a workgroup's share begins, and its walk from group to group
+struct Group {
+  int b, h, rb;      // sequence, key head, block of query rows
+  KvSeq q;
+  DecSeq d;
+  int64_t u0;        // the group's first unit
+};
+
+template <int KIND, int D, int RT>
+__global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
+  constexpr int NW = kWaves<D>, NT = 64 * NW, NS = Num<KIND>::NS, BR = 16 * RT;
+  constexpr int KC = D / 32;                       // products of 32 dims
+  constexpr int KG = KIND == kKvI8 ? KC / 2 : KC;  // granules of 16 keys
+  constexpr int DB = D / 16;
+  constexpr int VG = KIND == kKvI8 ? 1 : 2;        // granules of 16 dims
+  constexpr int BLK = kv_block_bytes(KIND, D);
+  constexpr bool F16 = KIND != kKvBf16;
+  constexpr float kLift = F16 ? 14.f : 0.f;
+  // LDS: the query parts [NS][RT][KC][64 lanes] granules; for the join the waves' sums [NW][BR][kJ + 4], in turns of kJ dims
+  constexpr int kJ = 32;
+  constexpr int kQBytes = NS * RT * KC * 1024, kJBytes = NW * BR * (kJ + 4) * 4;
+  extern __shared__ __align__(16) uint8_t lds[];
+  u32x4 *qf = (u32x4 *)lds;
+  float *js = (float *)lds;
+  __shared__ int64_t sum[NT / 64 + 4];
+  __shared__ float wm[NW][BR], wl[NW][BR], jf[NW][BR], jl[BR], jmax[BR];
+  __shared__ int flag;
+  __shared__ uint32_t qmax[BR];
+  static_assert(kQBytes <= 160 * 1024 && kJBytes <= 160 * 1024);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4,
+            col = lane & 15;
+  const int group = a.Hq / a.H;
+  auto load_q = [&](int64_t row, int c) {
+    return a.type == kRowF32    ? load8<kRowF32>(a.q, row, c)
+           : a.type == kRowBf16 ? load8<kRowBf16>(a.q, row, c)
+                                : load8<kRowF16>(a.q, row, c);
+  };
+  auto units = [&](int b) {
+    const DecSeq d = dec_seq(kv_seq(a.s, b), group, BR);
+    return (int64_t)d.pages * d.blocks * a.H;
+  };
+  // the share: all units first, then the place of the first (the scan again, over values that are now in the caches)
+  int64_t before = 0, all = 0;
+  find_item<NT>(a.s.n, -1, sum, &before, &all, units);
+  const int64_t share = dec_share(all, a.W, NW), u_lo = share * blockIdx.x, u_hi = min(u_lo + share, all);
+  if (u_lo >= u_hi) return;
+  Group g;
+  g.b = find_item<NT>(a.s.n, u_lo, sum, &before, &all, units);
+  g.q = kv_seq(a.s, g.b);
+  g.d = dec_seq(g.q, group, BR);
+  {
+    const int64_t in = u_lo - before;
+    const int64_t per_head = (int64_t)g.d.pages * g.d.blocks;
+    g.h = (int)(in / per_head);
+    g.rb = (int)(in % per_head / g.d.pages);
+    g.u0 = before + g.h * per_head + (int64_t)g.rb * g.d.pages;
+  }
+  int64_t u = u_lo;
+  for (;;) {  // one segment: the units [u, end) of group g
+    const int64_t g1 = g.u0 + g.d.pages, end = min(g1, u_hi);
+    const int pg0 = (int)(u - g.u0), pg1 = (int)(end - g.u0);
+    const int nrows = min(g.q.nr * group - g.rb * BR, BR);
+    __syncthreads();  // the segment before has left LDS
+    // ---- the block's query rows, scaled, in parts: granule (part, tile, chunk, lane) = 8 dims of row `col`
+    constexpr int QN = (RT * KC * 64 + NT - 1) / NT;
+    f32x8 x[QN];
+#pragma unroll
+    for (int n = 0; n < QN; n++) {
+      const int i = n * NT + tid, m = (i / (KC * 64)) * 16 + (i & 15), c = (i >> 6) % KC, qd = (i >> 4) & 3;
+      const int d = KIND == kKvI8 ? (c >> 1) * 64 + qd * 16 + (c & 1) * 8 : c * 32 + qd * 8;
+      if (i < RT * KC * 64 && m < nrows) {
+        const int row = g.rb * BR + m, t = row / group;
+        x[n] = load_q(g.q.r0 + t, (g.h * group + row - t * group) * D + d);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[n][k] = 0.f;
+      }
+    }
+    if constexpr (F16) {
+      if (tid < BR) qmax[tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < QN; n++) {
+        const int i = n * NT + tid;
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(x[n][k]) & 0x7FFFFFFFu);
+        if (i < RT * KC * 64) atomicMax(&qmax[(i / (KC * 64)) * 16 + (i & 15)], top);
+      }
+      __syncthreads();
+    }
+    auto q_exp = [&](int m) {  // the exponent taken out of row m
+      const uint32_t top = qmax[m];
+      return top == 0u || top >= 0x7F800000u ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(top));
+    };
+#pragma unroll
+    for (int n = 0; n < QN; n++) {
+      const int i = n * NT + tid;
+      if (i >= RT * KC * 64) break;
+      if constexpr (F16) {
+        const int e = -q_exp((i / (KC * 64)) * 16 + (i & 15));
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[n][k] = __builtin_amdgcn_ldexpf(x[n][k], e);
+      }
+#pragma unroll
+      for (int p = 0; p < NS; p++) qf[p * RT * KC * 64 + i] = part_of<KIND>(x[n]);
+    }
+    // the last token that row col of tile t sees
+    int seen[RT];
+    float scale[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      scale[t] = F16 ? __builtin_amdgcn_ldexpf(a.scale, q_exp(t * 16 + col)) : a.scale;
+      const int row = g.rb * BR + t * 16 + col;
+      seen[t] = t * 16 + col < nrows ? g.q.len - g.q.nr + row / group : -1;
+    }
+    const int all_see = g.q.len - g.q.nr + g.rb * BR / group;  // every row of the block sees up to here
+    __syncthreads();
+    f32x4 o[RT][DB];
+    float mx[RT], l[RT];
+    int ve = -200;  // 8 bits: the power of two that the sums are in units of (below any step's)
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      mx[t] = kNegInf;
+      l[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < DB; i++) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int *table = a.s.table + (int64_t)g.b * a.s.ldt;
+    for (int pg = pg0 + wave; pg < pg1; pg += NW) {
+      if (pg * kKvPage >= g.q.len) break;  // an empty sequence's only unit
+      const int id = __builtin_amdgcn_readfirstlane(table[pg]);
+      if (id < 0 || id >= a.s.pages) continue;
+      const uint8_t *blk = a.base + ((int64_t)id * a.H + g.h) * BLK;
+      const u32x4 *kp = (const u32x4 *)blk + lane, *vp = (const u32x4 *)(blk + kKvPage * D * kv_esize(KIND)) + lane;
+      u32x4 kf[4][KG], vf[DB][VG];
+#pragma unroll
+      for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+        for (int c = 0; c < KG; c++) kf[kb][c] = kp[(kb * KG + c) * 64];
+      auto load_values = [&] {
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+          for (int v = 0; v < VG; v++) vf[i][v] = vp[(i * VG + v) * 64];
+      };
+      if constexpr (RT == 1) load_values();
+      f32x4 ks[4], vs[4];
+      auto load_steps = [&] {
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++) {
+          ks[kb] = *(const f32x4 *)(blk + kv_step_at(D, 0, kb * 16 + quad * 4));
+          vs[kb] = *(const f32x4 *)(blk + kv_step_at(D, 1, kb * 16 + quad * 4));
+        }
+      };
+      if constexpr (KIND == kKvI8 && RT == 1) load_steps();
+      const bool edge = pg * kKvPage + kKvPage - 1 > all_see;  // some row does not see some key of the page
+      const int j0 = pg * kKvPage + quad * 4;
+      // ---- scores: lane (row col, keys kb * 16 + 4 quad + i)
+      f32x4 s[RT][4];
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++) s[t][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; c++) {
+        if constexpr (KIND == kKvI8 && RT > 1) __builtin_amdgcn_sched_barrier(0);  // (no conversions ahead: registers)
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int p = NS - 1; p >= 0; p--) {
+            const u32x4 b = qf[((p * RT + t) * KC + c) * 64 + lane];
+#pragma unroll
+            for (int kb = 0; kb < 4; kb++) {
+              u32x4 k;
+              if constexpr (KIND == kKvI8) {
+                const u32x4 w = kf[kb][c >> 1];
+                k = __builtin_bit_cast(u32x4, i8_f16((c & 1) ? u32x2{w[2], w[3]} : u32x2{w[0], w[1]}));
+              } else {
+                k = kf[kb][c];
+              }
+              s[t][kb] = mfma<KIND>(k, b, s[t][kb]);
+            }
+          }
+      }
+      float vshift = 1.f;
+      if constexpr (KIND == kKvI8 && RT > 1) load_steps();
+      if constexpr (KIND == kKvI8) {
+        float top = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if (edge && j0 + kb * 16 + i >= g.q.len) vs[kb][i] = 0.f;  // behind the last token a step may be anything
+            top = fmaxf(top, vs[kb][i]);
+          }
+        top = fmaxf(top, xor_lane<16>(top, lane));
+        top = fmaxf(top, xor_lane<32>(top, lane));
+        const int e = max(ve, top > 0.f ? __builtin_amdgcn_frexp_expf(top) : ve);
+        vshift = __builtin_amdgcn_ldexpf(1.f, ve - e);
+        ve = e;
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) vs[kb][i] = __builtin_amdgcn_ldexpf(vs[kb][i], -e);
+        }
+      }
+      if constexpr (RT > 1) load_values();  // (two row tiles leave no registers for both)
+      f32x8 p[RT][2];
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        float top = kNegInf;
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float v = s[t][kb][i] * scale[t];
+            if constexpr (KIND == kKvI8) v *= ks[kb][i];
+            if (edge) v = j0 + kb * 16 + i <= seen[t] ? v : kNegInf;
+            s[t][kb][i] = v;
+            top = fmaxf(top, v);
+          }
+        top = fmaxf(top, xor_lane<16>(top, lane));
+        top = fmaxf(top, xor_lane<32>(top, lane));
+        const float m1 = fmaxf(mx[t], top), ms = m1 == kNegInf ? 0.f : m1, ml = ms - kLift;
+        const float alpha = __builtin_amdgcn_exp2f(mx[t] - ms);
+        mx[t] = m1;
+        float add = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float e = __builtin_amdgcn_exp2f(s[t][kb][i] - ml);
+            add += e;
+            if constexpr (KIND == kKvI8) {
+              e *= vs[kb][i];
+              if (edge) e = j0 + kb * 16 + i <= seen[t] ? e : 0.f;  // (a step may be NaN)
+            }
+            p[t][kb >> 1][(kb & 1) * 4 + i] = e;
+          }
+        l[t] = l[t] * alpha + add;
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[t][i] *= alpha * vshift;
+      }
+      // 16 bits: what lies behind the last token may be anything, and 0 times it too, so it is cleared. Among drafts a value
+      // that is not finite must not reach the rows of earlier drafts either: it is taken out of the product, and the sums of
+      // the rows that see it are made NaN (which of them, the same product of ones tells).
+      bool odd = false;
+      auto kept = [&](u32x4 w, int kg) {  // the keys before len (recomputed where it is used: edges are rare, registers are not)
+        const int left = again(g.q.len - j0) - kg * 32;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int j = (k >> 1) * 16 + (k & 1) * 2;
+          w[k] &= (j < left ? 0xFFFFu : 0u) | (j + 1 < left ? 0xFFFF0000u : 0u);
+        }
+        return w;
+      };
+      if constexpr (KIND != kKvI8) {
+        if (edge && g.q.nr > 1) {
+          constexpr uint32_t e = KIND == kKvBf16 ? 0x7F80u : 0x7C00u;
+          uint32_t lo = 0, hi = 0;
+#pragma unroll
+          for (int i = 0; i < DB; i++)
+#pragma unroll
+            for (int kg = 0; kg < 2; kg++) {
+              const u32x4 w = kept(vf[i][kg], kg);
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                lo = max(lo, w[k] & e);
+                hi = max(hi, w[k] & e << 16);
+              }
+            }
+          odd = __ballot(lo == e || hi == e << 16) != 0;
+        }
+      }
+#pragma unroll
+      for (int kg = 0; kg < 2; kg++) {
+        __builtin_amdgcn_sched_barrier(0);  // (the groups one after the other: both at once take too many registers)
+        u32x4 pf[RT][NS];
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int k = 0; k < NS; k++) pf[t][k] = part_of<KIND>(p[t][kg]);
+#pragma unroll
+        for (int i = 0; i < DB; i++) {
+          u32x4 v;
+          if constexpr (KIND == kKvI8) {
+            const u32x4 w = vf[i][0];
+            v = __builtin_bit_cast(u32x4, i8_f16(kg ? u32x2{w[2], w[3]} : u32x2{w[0], w[1]}));
+          } else {
+            v = vf[i][kg];
+            if (edge) v = kept(v, kg);
+            if (__builtin_expect(odd, 0)) {
+              u32x4 one;
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                const uint32_t bad = not_finite<KIND>(v[k]);
+                one[k] = bad & (kOne<KIND> | kOne<KIND> << 16);
+                v[k] &= ~bad;
+              }
+#pragma unroll
+              for (int t = 0; t < RT; t++) {
+                const int last = again(seen[t] - j0) - kg * 32;
+                u32x4 sees;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                  const int j = (k >> 1) * 16 + (k & 1) * 2;
+                  sees[k] = (j <= last ? kOne<KIND> : 0u) | (j + 1 <= last ? kOne<KIND> << 16 : 0u);
+                }
+                const f32x4 n = mfma<KIND>(one, sees, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                  if (n[k] > 0.f) o[t][i][k] = __builtin_nanf("");
+              }
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int k = NS - 1; k >= 0; k--) o[t][i] = mfma<KIND>(v, pf[t][k], o[t][i]);
+        }
+      }
+    }
+    if constexpr (KIND == kKvI8) {
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[t][i][k] = __builtin_amdgcn_ldexpf(o[t][i][k], ve);
+    }
+    // ---- the segment's waves joined
+    const int used = min(NW, pg1 - pg0);  // waves that had a page
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      float s = l[t];
+      s += xor_lane<16>(s, lane);
+      s += xor_lane<32>(s, lane);
+      if (quad == 0) {
+        wm[wave][t * 16 + col] = mx[t];
+        wl[wave][t * 16 + col] = s;
+      }
+    }
+    __syncthreads();  // and every wave has read its query parts
+    const DecPart part = dec_part(g.u0, g1, share, (int)blockIdx.x);
+    float *slot = a.part + (int64_t)part.slot * dec_slot_floats(D);
+    if (tid < BR) {
+      float m = kNegInf, s = 0.f;
+      for (int w = 0; w < used; w++) m = fmaxf(m, wm[w][tid]);
+      const float ms = m == kNegInf ? 0.f : m;
+      for (int w = 0; w < used; w++) {
+        const float f = __builtin_amdgcn_exp2f(wm[w][tid] - ms);
+        jf[w][tid] = f;
+        s += wl[w][tid] * f;
+      }
+      jl[tid] = s == 0.f ? 0.f : 1.f / s;
+      if (part.parts > 1) {
+        st_cg(slot + BR * D + tid, m);
+        st_cg(slot + BR * D + BR + tid, s);
+      }
+    }
+    auto out_at = [&](int m, int d, float v) {  // one output element
+      const int row = g.rb * BR + m, t = row / group;
+      store1(a.out, a.type, g.q.r0 + t, (g.h * group + row - t * group) * D + d, v);
+    };
+#pragma unroll
+    for (int c = 0; c < D / kJ; c++) {
+      if (c) __syncthreads();
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < kJ / 16; i++)
+          *(f32x4 *)(js + (wave * BR + t * 16 + col) * (kJ + 4) + i * 16 + quad * 4) = o[t][c * (kJ / 16) + i];
+      __syncthreads();
+      for (int i = tid; i < BR * kJ; i += NT) {
+        const int m = i / kJ, d = i % kJ;
+        if (m >= nrows) break;
+        float s = 0.f;
+        for (int w = 0; w < used; w++) s = __builtin_fmaf(js[(w * BR + m) * (kJ + 4) + d], jf[w][m], s);
+        if (part.parts > 1) st_cg(slot + m * D + c * kJ + d, s);
+        else out_at(m, c * kJ + d, s * jl[m]);
+      }
+    }
+    // ---- the group's shares joined
+    if (part.parts > 1) {
+      __builtin_amdgcn_s_waitcnt(0);  // this wave's partials have arrived
+      __syncthreads();
+      if (tid == 0) flag = (int)atomicAdd(a.cnt + part.first, 1u);
+      __syncthreads();
+      if (flag == part.parts - 1) {
+        const float *base = a.part + (int64_t)part.first * 2 * dec_slot_floats(D);
+        // the first share's slot is its second if the group begins inside it; the others' their first
+        auto at = [&](int k) { return base + (int64_t)(2 * k + (k == 0 && g.u0 % share != 0 ? 1 : 0)) * dec_slot_floats(D); };
+        if (tid < nrows) {
+          float m = kNegInf;
+          for (int k = 0; k < part.parts; k++) m = fmaxf(m, ld_cg(at(k) + BR * D + tid));
+          const float ms = m == kNegInf ? 0.f : m;
+          float s = 0.f;
+          for (int k = 0; k < part.parts; k++)
+            s = __builtin_fmaf(ld_cg(at(k) + BR * D + BR + tid), __builtin_amdgcn_exp2f(ld_cg(at(k) + BR * D + tid) - ms), s);
+          jmax[tid] = ms;
+          jl[tid] = s == 0.f ? 0.f : 1.f / s;
+        }
+        __syncthreads();
+        for (int i = tid; i < nrows * D; i += NT) {
+          const int m = i / D, d = i % D;
+          float s = 0.f;
+          for (int k = 0; k < part.parts; k++)
+            s = __builtin_fmaf(ld_cg(at(k) + m * D + d), __builtin_amdgcn_exp2f(ld_cg(at(k) + BR * D + m) - jmax[m]), s);
+          out_at(m, d, s * jl[m]);
+        }
+        if (tid == 0) st_cg(a.cnt + part.first, 0u);
+      }
+    }
+    if (end == u_hi) return;
+    // ---- the next group
+    u = end;
+    g.u0 = end;
+    if (++g.rb == g.d.blocks) {
+      g.rb = 0;
+      if (++g.h == a.H) {
+        g.h = 0;
+        do {
+          if (++g.b >= a.s.n) return;  // (not reached: u < all, so a later sequence has rows)
+          g.q = kv_seq(a.s, g.b);
+          g.d = dec_seq(g.q, group, BR);
+        } while (!g.d.blocks);
+      }
+    }
+  }
+}
+
+template <int KIND, int D, int RT>
+constexpr int lds_bytes() {
+  constexpr int q = Num<KIND>::NS * RT * (D / 32) * 1024, j = kWaves<D> * 16 * RT * 36 * 4;
+  return q > j ? q : j;
+}
+
+template <typename F>
+void each(F &&f) {  // every instance
+  auto dims = [&](auto kind) {
+    auto rows = [&](auto dim) {
+      f(kind, dim, std::integral_constant<int, 1>());
+      f(kind, dim, std::integral_constant<int, 2>());
+    };
+    rows(std::integral_constant<int, 64>());
+    rows(std::integral_constant<int, 128>());
+    rows(std::integral_constant<int, 256>());
+  };
+  dims(std::integral_constant<int, kKvBf16>());
+  dims(std::integral_constant<int, kKvF16>());
+  dims(std::integral_constant<int, kKvI8>());
+}
+
+}  // namespace
+
+int decode_grid() {
+  int dev = 0, cus = 0;
+  IJ_HIP(hipGetDevice(&dev));
+  IJ_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+  return cus;
+}
+
+void launch_attn_decode(const DecArgs &a, hipStream_t s) {
+  // 16 query rows a block while a token's rows fill no more than that, else 32: each block reads the pages once
+  const int rt = a.Hq / a.H <= 16 && a.s.R <= a.s.n ? 1 : 2;
+  each([&](auto kind, auto dim, auto tiles) {
+    if (a.kind == kind && a.D == dim && rt == tiles)
+      hipLaunchKernelGGL((attn_decode<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>), dim3(a.W),
+                         dim3(64 * kWaves<decltype(dim)::value>),
+                         (lds_bytes<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>()), s, a);
+  });
+  IJ_HIP(hipGetLastError());
+}
+
+void init_decode_attrs() {
+  each([&](auto kind, auto dim, auto tiles) {
+    IJ_HIP(hipFuncSetAttribute(
+        (const void *)attn_decode<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>,
+        hipFuncAttributeMaxDynamicSharedMemorySize,
+        lds_bytes<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>()));
+  });
+}
+
+}  // namespace ijah

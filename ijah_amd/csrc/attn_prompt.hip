@@ -1,0 +1,334 @@
+// Causal attention over packed prompts with grouped heads: out_i = sum_{j <= i + nk - nq} softmax_j(scale q_i . k_j) v_j.
+//
+// One pass over a block's keys with the running maximum and sum of each row (f32, base 2: the scale carries log2 e). Bound
+// by the matrix cores and the softmax beside them: 4 D products and about 5 vector operations (one of them an exponential
+// at a quarter of the rate) per visible pair.
+//
+// A workgroup of four waves takes 128 query rows of one head of one sequence, a wave 32 of them; tiles of BN keys and
+// values go through LDS. S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16: a lane holds one query row, so its maximum
+// needs one lane swap, and the weights that the product of the keys leaves in a lane are those the product of the values
+// wants there once the keys of its A operand are taken in the same order (4 half + {0..3}, 8 + 4 half + {0..3}), which
+// ds_read_b64_tr_b16 reads transposed from the rows of V.
+//
+// 32-bit rows are cut into NT = 3 bf16 parts (8 bits each) and each product is the sum of the six part products that
+// reach 2^-24: exact to f32's own rounding at six times the matrix work, with f32's range. 16-bit rows are products of
+// their own type (NT = 1), the weights rounded to it (2^-9 or 2^-12 of each, as the output itself); sums are f32.
+#include "attn_device.h"
+#include "common.h"
+
+namespace ijah {
+
+namespace {
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr int kBM = 128;  // query rows of a workgroup
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// x = part + rest exactly, the part in bf16
+__device__ __forceinline__ u32x4 bf16_part(f32x8 &x) {
+  const u32x4 w = to_bf16x8(x);
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    x[2 * k] -= __uint_as_float(w[k] << 16);
+    x[2 * k + 1] -= __uint_as_float(w[k] & 0xFFFF0000u);
+  }
+  return w;
+}
+
+// Where 16-byte chunk c (8 dims) of tile row j lies in LDS, in chunks. Keys are read 32 rows of one chunk at a time, so rows
+// are rotated over all chunks of 256 bytes; values are read 4 rows of a pair of chunks at a time per 16 lanes, so pairs
+// stay together and four consecutive rows spread over different pairs.
+template <int D>
+__device__ __forceinline__ int key_chunk(int j, int c) {
+  return j * (D / 8) + (c ^ (D == 64 ? (j >> 1) & 7 : j & 15));
+}
+template <int D>
+__device__ __forceinline__ int value_chunk(int j, int c) {
+  return j * (D / 8) + (c ^ (D == 64 ? (((j >> 1) & 1) << 1 | ((j >> 2) & 1)) << 1 : ((j & 3) << 1 | ((j >> 2) & 1)) << 1));
+}
+
+template <int D, int BN, int NT, bool F16>
+__global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
+  constexpr int KC = D / 16, DB = D / 32, KB = BN / 32, CH = D / 8, kPlane = BN * D * 2;
+  extern __shared__ __align__(16) uint8_t lds[];  // keys [NT][BN][D], values [NT][BN][D]
+  __shared__ int64_t sum[8];
+  __shared__ uint32_t odd[BN];  // keys of the tile whose value is not finite
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5,
+            col = lane & 31;
+  auto bound = [](const int *p, int b, int R) { return kv_clamp(p[b], 0, R); };
+  auto q_of = [&](int b) { return max(bound(a.q_rows, b + 1, a.Rq) - bound(a.q_rows, b, a.Rq), 0); };
+  int64_t before = 0, all = 0;
+  // the last blocks see the most keys: they go first
+  const int64_t blocks = gridDim.x / a.Hq;
+  const int h = blockIdx.x % a.Hq;
+  const int64_t item = blocks - 1 - blockIdx.x / a.Hq;
+  const int b = find_item<256>(a.n, item, sum, &before, &all, [&](int i) { return (int64_t)((q_of(i) + kBM - 1) / kBM); });
+  if (b < 0) return;
+  const int nq = q_of(b), q0 = bound(a.q_rows, b, a.Rq), i0 = (int)(item - before) * kBM;
+  const int k0 = bound(a.k_rows, b, a.Rk), nk = max(bound(a.k_rows, b + 1, a.Rk) - k0, 0);
+  const int off = nk - nq, hk = h / (a.Hq / a.H);
+  const int row = i0 + wave * 32 + col;  // this lane's query row in its sequence
+  const int last = row + off;            // the last key it sees
+  const int keys = min(nk, min(i0 + kBM, nq) + off);  // of the block
+  const int all_see = i0 + off;                       // every row sees up to here
+
+  // the wave's query rows as B operands; three parts of 256 dims are cut again for each tile (192 registers otherwise)
+  constexpr bool kCut = NT == 3 && D == 256;
+  u32x4 qf[kCut ? 1 : NT][kCut ? 1 : KC];
+  f32x8 q32[kCut ? KC : 1];
+#pragma unroll
+  for (int c = 0; c < KC; c++) {
+    const int64_t r = q0 + min(row, nq - 1);
+    if constexpr (kCut) {
+      q32[c] = load8<kRowF32>(a.q, r, h * D + c * 16 + half * 8);
+    } else if constexpr (NT == 3) {
+      f32x8 x = load8<kRowF32>(a.q, r, h * D + c * 16 + half * 8);
+#pragma unroll
+      for (int p = 0; p < 3; p++) qf[p][c] = bf16_part(x);
+    } else {
+      qf[0][c] = *(const u32x4 *)((const uint16_t *)a.q.p + r * a.q.ld + h * D + c * 16 + half * 8);
+    }
+  }
+  f32x16 o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; i++)
+#pragma unroll
+    for (int k = 0; k < 16; k++) o[i][k] = 0.f;
+  float mx = kNegInf, l = 0.f;
+
+  for (int t0 = 0; t0 < keys; t0 += BN) {
+    const bool edge = t0 + BN - 1 > all_see || t0 + BN > nk;  // some row does not see some key of the tile
+    __syncthreads();
+    // ---- the tile into LDS; rows behind the sequence's last key are copies of it. In a tile whose keys not every row
+    // sees, a value that is not finite is cleared (0 times it is not 0) and remembered.
+    if (edge && tid < BN) odd[tid] = 0;
+    if (edge) __syncthreads();
+#pragma unroll(NT == 3 ? 2 : BN * CH / 256)
+    for (int n = 0; n < BN * CH / 256; n++) {
+      const int i = n * 256 + tid, j = i / CH, c = i % CH;
+      const int64_t r = k0 + min(t0 + j, nk - 1);
+      if constexpr (NT == 3) {
+        f32x8 x = load8<kRowF32>(a.k, r, hk * D + c * 8);
+        f32x8 y = load8<kRowF32>(a.v, r, hk * D + c * 8);
+        if (edge) {
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if ((__float_as_uint(y[k]) & 0x7F800000u) == 0x7F800000u) {
+              y[k] = 0.f;
+              if (t0 + j < nk) odd[j] = 1;
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+          *(u32x4 *)(lds + p * kPlane + key_chunk<D>(j, c) * 16) = bf16_part(x);
+          *(u32x4 *)(lds + (3 + p) * kPlane + value_chunk<D>(j, c) * 16) = bf16_part(y);
+        }
+      } else {
+        const u32x4 x = *(const u32x4 *)((const uint16_t *)a.k.p + r * a.k.ld + hk * D + c * 8);
+        u32x4 y = *(const u32x4 *)((const uint16_t *)a.v.p + r * a.v.ld + hk * D + c * 8);
+        if (edge) {
+          constexpr uint32_t e = F16 ? 0x7C00u : 0x7F80u;
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t bad = ((y[k] & e) == e ? 0xFFFFu : 0u) | ((y[k] >> 16 & e) == e ? 0xFFFF0000u : 0u);
+            y[k] &= ~bad;
+            if (bad && t0 + j < nk) odd[j] = 1;
+          }
+        }
+        *(u32x4 *)(lds + key_chunk<D>(j, c) * 16) = x;
+        *(u32x4 *)(lds + kPlane + value_chunk<D>(j, c) * 16) = y;
+      }
+    }
+    __syncthreads();
+    // ---- scores: lane (row col, keys 32 kb + 8 (i / 4) + 4 half + i % 4)
+    f32x16 s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int k = 0; k < 16; k++) s[kb][k] = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int c = 0; c < KC; c++) {
+        u32x4 kf[NT], qc[NT];
+        if constexpr (kCut) {
+          f32x8 x = q32[c];
+          asm volatile("" : "+v"(x));
+#pragma unroll
+          for (int p = 0; p < NT; p++) qc[p] = bf16_part(x);
+        } else {
+#pragma unroll
+          for (int p = 0; p < NT; p++) qc[p] = qf[p][c];
+        }
+#pragma unroll
+        for (int p = 0; p < NT; p++)
+          kf[p] = *(const u32x4 *)(lds + p * kPlane + key_chunk<D>(kb * 32 + col, c * 2 + half) * 16);
+        if constexpr (NT == 3) {  // smallest products first
+          s[kb] = mfma32<F16>(kf[2], qc[0], s[kb]);
+          s[kb] = mfma32<F16>(kf[0], qc[2], s[kb]);
+          s[kb] = mfma32<F16>(kf[1], qc[1], s[kb]);
+          s[kb] = mfma32<F16>(kf[1], qc[0], s[kb]);
+          s[kb] = mfma32<F16>(kf[0], qc[1], s[kb]);
+        }
+        s[kb] = mfma32<F16>(kf[0], qc[0], s[kb]);
+      }
+    float top = kNegInf;
+    const int seen = last - t0 - 4 * half;
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        if (edge && kb * 32 + (i >> 2) * 8 + (i & 3) > min(seen, nk - 1 - t0 - 4 * half)) s[kb][i] = kNegInf;
+        top = fmaxf(top, s[kb][i]);
+      }
+    top = fmaxf(top, xor_lane<32>(top, lane));
+    const float m1 = fmaxf(mx, top), ms = m1 == kNegInf ? 0.f : m1 * a.scale;
+    const float alpha = __builtin_amdgcn_exp2f(mx == kNegInf ? kNegInf : __builtin_fmaf(mx, a.scale, -ms));
+    mx = m1;
+    float add = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.scale, -ms));
+        add += e;
+        s[kb][i] = e;
+      }
+    l = __builtin_fmaf(l, alpha, add);
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] *= alpha;
+    // ---- sums
+#pragma unroll
+    for (int kg = 0; kg < BN / 16; kg++) {
+      u32x4 pf[NT];
+      f32x8 p;
+#pragma unroll
+      for (int k = 0; k < 8; k++) p[k] = s[kg >> 1][(kg & 1) * 8 + k];
+      if constexpr (NT == 3) {
+#pragma unroll
+        for (int k = 0; k < 3; k++) pf[k] = bf16_part(p);
+      } else {
+        pf[0] = F16 ? to_f16x8(p) : to_bf16x8(p);
+      }
+#pragma unroll
+      for (int i = 0; i < DB; i++) {
+        u32x4 vf[NT];
+#pragma unroll
+        for (int k = 0; k < NT; k++) {
+          // 16 lanes read 4 keys x 16 dims and get 4 keys of one dim each
+          const int j = kg * 16 + half * 4 + ((lane & 15) >> 2), c = i * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+          uint8_t *base = lds + (NT + k) * kPlane + (lane & 1) * 8;
+          auto tr = [&](int jj) {
+            return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4 *)(base + value_chunk<D>(jj, c) * 16)));
+          };
+          const u32x2 v0 = tr(j), v1 = tr(j + 8);
+          vf[k] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+        }
+        if constexpr (NT == 3) {
+          o[i] = mfma32<F16>(vf[2], pf[0], o[i]);
+          o[i] = mfma32<F16>(vf[0], pf[2], o[i]);
+          o[i] = mfma32<F16>(vf[1], pf[1], o[i]);
+          o[i] = mfma32<F16>(vf[1], pf[0], o[i]);
+          o[i] = mfma32<F16>(vf[0], pf[1], o[i]);
+        }
+        o[i] = mfma32<F16>(vf[0], pf[0], o[i]);
+      }
+    }
+    // ---- rows that see a value that is not finite
+    if (edge) {
+      for (int j = 0; j < min(BN, nk - t0); j++) {
+        if (!odd[j] || t0 + j > last) continue;
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+          for (int k = 0; k < 16; k++) {
+            const int64_t at = (int64_t)(k0 + t0 + j) * a.v.ld + hk * D + i * 32 + (k >> 2) * 8 + half * 4 + (k & 3);
+            const float v = NT == 3 ? ((const float *)a.v.p)[at]
+                            : F16   ? (float)((const _Float16 *)a.v.p)[at]
+                                    : bf16_f32(((const uint16_t *)a.v.p)[at]);
+            if ((__float_as_uint(v) & 0x7F800000u) == 0x7F800000u) o[i][k] = __builtin_nanf("");
+          }
+      }
+    }
+  }
+  l += xor_lane<32>(l, lane);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (row < nq) {
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int64_t at = (q0 + row) * a.out.ld + h * D + i * 32 + k * 8 + half * 4;
+        const f32x4 v = {o[i][4 * k] * inv, o[i][4 * k + 1] * inv, o[i][4 * k + 2] * inv, o[i][4 * k + 3] * inv};
+        if constexpr (NT == 3) {
+          *(f32x4 *)((float *)a.out.p + at) = v;
+        } else if constexpr (F16) {
+          f16x4 w;
+#pragma unroll
+          for (int x = 0; x < 4; x++) w[x] = (_Float16)v[x];
+          *(f16x4 *)((_Float16 *)a.out.p + at) = w;
+        } else {
+          typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+          bf16x4 w;
+#pragma unroll
+          for (int x = 0; x < 4; x++) w[x] = (__bf16)v[x];
+          *(bf16x4 *)((__bf16 *)a.out.p + at) = w;
+        }
+      }
+  }
+}
+
+// keys of a tile: what three planes of 256 dims leave room for in LDS
+template <int D, int NT>
+constexpr int kBN = D == 256 && NT == 3 ? 32 : 64;
+
+template <typename F>
+void each(F &&f) {  // every instance: dims, parts, fp16
+  auto dims = [&](auto nt, auto f16) {
+    f(std::integral_constant<int, 64>(), nt, f16);
+    f(std::integral_constant<int, 128>(), nt, f16);
+    f(std::integral_constant<int, 256>(), nt, f16);
+  };
+  dims(std::integral_constant<int, 3>(), std::false_type());
+  dims(std::integral_constant<int, 1>(), std::false_type());
+  dims(std::integral_constant<int, 1>(), std::true_type());
+}
+template <int D, int NT>
+constexpr int prompt_lds() {
+  return 2 * NT * kBN<D, NT> * D * 2;
+}
+
+}  // namespace
+
+void launch_attn_prompt(const PromptArgs &a, hipStream_t s) {
+  const int64_t blocks = std::min<int64_t>(a.Rq, a.Rq / kBM + a.n);  // a sequence's last block may be partial
+  each([&](auto dim, auto nt, auto f16) {
+    constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
+    constexpr bool F16 = decltype(f16)::value;
+    if (a.D == D && a.type == (NT == 3 ? kRowF32 : F16 ? kRowF16 : kRowBf16))
+      hipLaunchKernelGGL((attn_prompt<D, kBN<D, NT>, NT, F16>), dim3((unsigned)(blocks * a.Hq)), dim3(256),
+                         (prompt_lds<D, NT>()), s, a);
+  });
+  IJ_HIP(hipGetLastError());
+}
+
+void init_decode_attrs();
+void init_attn_attrs() {
+  init_decode_attrs();
+  each([&](auto dim, auto nt, auto f16) {
+    constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
+    IJ_HIP(hipFuncSetAttribute((const void *)attn_prompt<D, kBN<D, NT>, NT, decltype(f16)::value>,
+                               hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<D, NT>()));
+  });
+}
+
+}  // namespace ijah

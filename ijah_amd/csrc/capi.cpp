@@ -40,6 +40,12 @@ bool device_available() {
   return avail == 1;
 }
 
+static std::vector<void (*)()> &setup_hooks() {
+  static std::vector<void (*)()> hooks;
+  return hooks;
+}
+void on_device_setup(void (*f)()) { setup_hooks().push_back(f); }
+
 void ensure_device() {
   static std::once_flag once;
   static std::string err;
@@ -54,6 +60,7 @@ void ensure_device() {
       init_fused_attrs();
       init_lin_attrs();
       noalloc_scratch();  // the allocation-free linear's scratch address on this device
+      for (auto f : setup_hooks()) f();
     } catch (const std::exception &e) {
       err = e.what();
     }

@@ -50,6 +50,9 @@ int c_call(F &&f) {
 // The library's stream: every entry point enqueues here; synchronous entry points wait on it.
 hipStream_t stream();
 void ensure_device();
+// f runs once at device set-up, before any launch and so before any stream capture (kernel attributes); sources that the
+// host-only builds leave out register here instead of being named there. Call it while the library loads.
+void on_device_setup(void (*f)());
 bool device_available();  // a HIP device is visible (no throw)
 
 // the caller's pending mirror writes of b pushed to the device (not while the library stream is captured), then

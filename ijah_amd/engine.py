@@ -79,6 +79,23 @@ class MoeHc(C.Structure):  # ne_moe_hc: the hyper-connection write fused into th
     _fields_ = [("hc", C.c_int), ("refr", C.c_int), ("h", C.c_void_p), ("inj", C.c_void_p), ("hout", C.c_void_p)]
 
 
+KV_PAGE = 64  # NE_KV_PAGE: tokens of a cache page
+
+
+class KvDesc(C.Structure):  # ne_kv_desc
+    _fields_ = [(n, C.c_int) for n in ("layers", "pages", "heads", "dim", "dtype")]
+
+
+class KvSeqsC(C.Structure):  # ne_kv_seqs
+    _fields_ = [("n", C.c_int), ("ldt", C.c_int), ("table", C.c_void_p), ("lens", C.c_void_p), ("rows", C.c_void_p)]
+
+
+class AttnPromptC(C.Structure):  # ne_attn_prompt_desc
+    _fields_ = ([(n, C.c_int) for n in ("n", "heads", "kv_heads", "dim", "dtype", "Rq", "Rk", "ldq", "ldk", "ldv", "ldo")] +
+                [("scale", C.c_float)] + [(n, C.c_void_p) for n in ("q_rows", "k_rows", "q", "k", "v")] +
+                [(n, C.c_uint64) for n in ("q_off", "k_off", "v_off", "out_off")] + [("out", C.c_void_p)])
+
+
 class EngineError(RuntimeError):
     pass
 
@@ -122,6 +139,13 @@ SIGNATURES = {
     "ne_moe_info": (_i, [_vp] + [_ip] * 6), "ne_moe_bytes": (_i, [_vp, _i, C.POINTER(_u64)]),
     "ne_moe_time": (_i, [C.POINTER(_vp), _i, _i, _vp, _i, _i, _dp]),
     "ne_moe_time_kernels": (_i, [C.POINTER(_vp), _i, _i, _vp, _i, _vp, _dp, _ip]),
+    # include/ijah_attn.h
+    "ne_kv_create": (_vp, [C.POINTER(KvDesc)]), "ne_kv_free": (None, [_vp]),
+    "ne_kv_info": (_i, [_vp, C.POINTER(KvDesc), C.POINTER(_u64)]),
+    "ne_kv_write": (_i, [_vp, _i, C.POINTER(KvSeqsC), _i, _vp, _u64, _i, _vp, _u64, _i, _i, _dp]),
+    "ne_kv_read": (_i, [_vp, _i, C.POINTER(KvSeqsC), _i, _vp, _u64, _i, _vp, _u64, _i, _i, _dp]),
+    "ne_attn_decode": (_i, [_vp, _i, C.POINTER(KvSeqsC), _i, _i, _vp, _u64, _i, _vp, _u64, _i, _i, C.c_float, _dp]),
+    "ne_attn_prompt": (_i, [C.POINTER(AttnPromptC), _dp]),
 }
 
 
@@ -388,6 +412,78 @@ class MoeLayer(_Handle):
         return b.value
 
 
+# ---------------------------------------------------------------------------------------------- attention
+_DTYPE_CODE = {n: c for c, n in DTYPES.items()}
+
+
+def _rows_dtype(dtype):
+    if dtype not in ("F32", "BF16", "F16"):
+        raise EngineError(f"rows of type {dtype} (F32, BF16 or F16)")
+    return _DTYPE_CODE[dtype]
+
+
+class KvSeqs:
+    """A batch of sequences over a cache (ne_kv_seqs), its tables on the device: table i32 [n][ldt] page ids, lens i32 [n]
+    tokens after the step, rows i32 [n + 1] each sequence's rows of the call (None: one row each)."""
+
+    def __init__(self, n, ldt, table, lens, rows=None):
+        self.n, self.ldt, self.table, self.lens, self.rows = n, ldt, table, lens, rows
+        self.c = KvSeqsC(n, ldt, table.ptr, lens.ptr, rows.ptr if rows is not None else None)
+
+
+class KvCache(_Handle):
+    """A paged key-value cache of several layers (ne_kv_*), and the attention of new tokens over it."""
+    _release = "ne_kv_free"
+
+    def __init__(self, eng, ptr):
+        super().__init__(eng, ptr)
+        d, b = KvDesc(), C.c_uint64(0)
+        self._call("ne_kv_info", C.byref(d), C.byref(b))
+        self.layers, self.pages, self.heads, self.dim, self.nbytes = d.layers, d.pages, d.heads, d.dim, b.value
+        self.dtype = DTYPES[d.dtype]
+
+    def _rows(self, name, layer, seqs, R, k, v, dtype, k_off, v_off, ldk, ldv, timed):
+        ms = C.c_double(0)
+        self._call(name, layer, C.byref(seqs.c), R, k.ptr, k_off, ldk, v.ptr, v_off, ldv, _rows_dtype(dtype),
+                   _ms_arg(timed, ms))
+        return ms.value
+
+    def write_bufs(self, layer, seqs, R, k, v, dtype="F32", k_off=0, v_off=0, ldk=0, ldv=0, timed=False):
+        """ne_kv_write: the R rows k, v (device buffers) become the sequences' newest tokens"""
+        return self._rows("ne_kv_write", layer, seqs, R, k, v, dtype, k_off, v_off, ldk, ldv, timed)
+
+    def read_bufs(self, layer, seqs, R, k, v, dtype="F32", k_off=0, v_off=0, ldk=0, ldv=0, timed=False):
+        """ne_kv_read: the same tokens back as rows"""
+        return self._rows("ne_kv_read", layer, seqs, R, k, v, dtype, k_off, v_off, ldk, ldv, timed)
+
+    def attend_bufs(self, layer, seqs, R, heads, q, out, dtype="F32", scale=None, q_off=0, out_off=0, ldq=0, ldo=0,
+                    timed=False):
+        """ne_attn_decode: attention of the R newest tokens over the cache; scale None: 1 / sqrt(dim)"""
+        ms = C.c_double(0)
+        self._call("ne_attn_decode", layer, C.byref(seqs.c), R, heads, q.ptr, q_off, ldq, out.ptr, out_off, ldo,
+                   _rows_dtype(dtype), self.dim ** -0.5 if scale is None else scale, _ms_arg(timed, ms))
+        return ms.value
+
+    def write(self, layer, seqs, k, v):
+        """f32 arrays [R][heads][dim]"""
+        k, v = (np.ascontiguousarray(x, np.float32) for x in (k, v))
+        self.write_bufs(layer, seqs, k.shape[0], self.eng.from_numpy(k), self.eng.from_numpy(v))
+        self.eng.sync()  # the rows' buffers go with this call
+
+    def read(self, layer, seqs, R):
+        shape = (R, self.heads, self.dim)
+        b = [self.eng.alloc(int(np.prod(shape)) * 4) for _ in range(2)]
+        self.read_bufs(layer, seqs, R, *b)
+        return [x.download(np.float32, shape) for x in b]
+
+    def attend(self, layer, seqs, q, scale=None):
+        """q f32 [R][heads][dim] -> f32 of its shape"""
+        q = np.ascontiguousarray(q, np.float32)
+        qb, ob = self.eng.from_numpy(q), self.eng.alloc(q.nbytes)
+        self.attend_bufs(layer, seqs, q.shape[0], q.shape[1], qb, ob, scale=scale)
+        return ob.download(np.float32, q.shape)
+
+
 # ---------------------------------------------------------------------------------------------- kernel arguments
 def _arg_buf(a):
     return ArgC(a.ptr, 0, None, 0), None
@@ -598,3 +694,35 @@ class Engine:
         self._ok(self.lib.ne_moe_time_kernels(_ptrs(layers), len(layers), R, x.ptr, reps, names, us, C.byref(n)),
                  "ne_moe_time_kernels")
         return {names[i].value.decode(): us[i] for i in range(n.value)}
+
+    # ---- attention
+    def kv_create(self, layers, pages, heads, dim, dtype="BF16"):
+        """a paged key-value cache (ne_kv_create); dtype BF16, F16 or I8"""
+        d = KvDesc(layers, pages, heads, dim, _DTYPE_CODE.get(dtype, -1))
+        return KvCache(self, self._made(self.lib.ne_kv_create(C.byref(d)), "ne_kv_create"))
+
+    def kv_seqs(self, table, lens, rows=None):
+        """KvSeqs of host arrays: table [n][ldt], lens [n], rows [n + 1] or None"""
+        table = np.atleast_2d(np.asarray(table, np.int32))
+        b = [None if x is None else self.from_numpy(np.asarray(x, np.int32)) for x in (table, lens, rows)]
+        return KvSeqs(table.shape[0], table.shape[1], *b)
+
+    def attn_prompt_bufs(self, n, q_rows, k_rows, Rq, Rk, heads, kv_heads, dim, q, k, v, out, dtype="F32", scale=None,
+                         q_off=0, k_off=0, v_off=0, out_off=0, ldq=0, ldk=0, ldv=0, ldo=0, timed=False):
+        """ne_attn_prompt on device buffers; k_rows None: q_rows; scale None: 1 / sqrt(dim)"""
+        d = AttnPromptC(n, heads, kv_heads, dim, _rows_dtype(dtype), Rq, Rk, ldq, ldk, ldv, ldo,
+                        dim ** -0.5 if scale is None else scale, q_rows.ptr, k_rows.ptr if k_rows is not None else None,
+                        q.ptr, k.ptr, v.ptr, q_off, k_off, v_off, out_off, out.ptr)
+        ms = C.c_double(0)
+        self._ok(self.lib.ne_attn_prompt(C.byref(d), _ms_arg(timed, ms)), "ne_attn_prompt")
+        return ms.value
+
+    def attn_prompt(self, q, k, v, q_rows, k_rows=None, scale=None):
+        """f32 arrays: q [Rq][heads][dim], k, v [Rk][kv_heads][dim]; q_rows, k_rows [n + 1]"""
+        q, k, v = (np.ascontiguousarray(x, np.float32) for x in (q, k, v))
+        qr = self.from_numpy(np.asarray(q_rows, np.int32))
+        kr = None if k_rows is None else self.from_numpy(np.asarray(k_rows, np.int32))
+        qb, kb, vb, ob = self.from_numpy(q), self.from_numpy(k), self.from_numpy(v), self.alloc(q.nbytes)
+        self.attn_prompt_bufs(len(q_rows) - 1, qr, kr, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], qb, kb,
+                              vb, ob, scale=scale)
+        return ob.download(np.float32, q.shape)
