@@ -85,34 +85,45 @@ IJ_HD int64_t kv_max_pieces(int n, int R, bool rows) {
 
 // ------------------------------------------------------------------------------------------------ decode's work
 // The batch's work in units of one page for one key head and one block of query rows, in the order (sequence, key head, row
-// block, page); every sequence with rows has at least one unit per head and block (an empty one writes its zeros). The W
-// workgroups take equal consecutive shares, whatever the lengths: share = max(kDecMin, ceil(units / W)) units. A (sequence,
-// head, block) that lies in several shares is joined by the last of them to finish, from one partial each: workgroup w's
-// first segment in slot 2w, one that begins inside its share in 2w + 1. At most one group that is continued begins in a
-// share, so its first workgroup's number names the counter.
+// block, page); every sequence with rows has at least one unit per head and block (an empty one writes its zeros). A (sequence,
+// head, block) is a group. The W workgroups take consecutive shares, in one of two forms:
+//   - few units: each group is filled up to a multiple of `least` units (a page for every wave of a workgroup), and a share is
+//     `least` of them, so that no workgroup has more than one group's, and none more than a page per wave;
+//   - else equal shares of ceil(units / W), whatever the lengths.
+// A group that lies in several shares is joined from one partial each: workgroup w's first segment is in slot 2w, one that
+// begins inside its share in 2w + 1. Parts are joined kJoin at a time by the last of them to finish, into the first one's slot
+// (whose number names the counter), and these by the last of their joins (at most one group that is continued begins in a
+// share, so its first workgroup names that counter): one workgroup reading all of a long sequence's parts would take longer
+// than its pages do.
 struct DecSeq {
-  int pages, blocks;  // units per head: pages * blocks
+  int pages, blocks;  // pages (at least one), row blocks
 };
 IJ_HD DecSeq dec_seq(const KvSeq &q, int group, int block_rows) {
   DecSeq d;
   d.pages = q.len > 0 ? (q.len + kKvPage - 1) / kKvPage : 1;
-  d.blocks = (int)(((int64_t)q.nr * group + block_rows - 1) / block_rows);
+  d.blocks = (q.nr * group + block_rows - 1) / block_rows;
   return d;
 }
-IJ_HD int64_t dec_share(int64_t units, int W, int least) {
-  const int64_t c = (units + W - 1) / W;
-  return c > least ? c : least;
+IJ_HD int dec_units(const DecSeq &d, int H, int pad) { return (d.pages + pad - 1) / pad * pad * d.blocks * H; }
+// the most units that a batch can have, filled up: the host refuses batches where this passes 31 bits
+IJ_HD int64_t dec_max_units(int n, int ldt, int R, int group, int H, int block_rows, int pad) {
+  return ((int64_t)R * group / block_rows + n) * H * ((int64_t)ldt + pad);
 }
+constexpr int kJoin = 16;
 struct DecPart {
   int first, parts, slot;  // the group's first workgroup, how many it has, this one's partial slot
 };
 // the group of units [g0, g1) seen from workgroup w
-IJ_HD DecPart dec_part(int64_t g0, int64_t g1, int64_t share, int w) {
+IJ_HD DecPart dec_part(int g0, int g1, int share, int w) {
   DecPart p;
-  p.first = (int)(g0 / share);
-  p.parts = (int)((g1 - 1) / share) - p.first + 1;
-  p.slot = 2 * w + (w == p.first && g0 % share != 0 ? 1 : 0);
+  p.first = g0 / share;
+  p.parts = (g1 - 1) / share - p.first + 1;
+  p.slot = 2 * w + (w == p.first && g0 != p.first * share ? 1 : 0);
   return p;
+}
+// part k's slot
+IJ_HD int dec_slot(const DecPart &p, int g0, int share, int k) {
+  return 2 * (p.first + k) + (k == 0 && g0 != p.first * share ? 1 : 0);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -136,7 +147,7 @@ struct DecArgs {
   int type;
   float scale;     // times log2 e
   float *part;     // [2 W] slots of dec_slot_floats
-  uint32_t *cnt;   // [W], zero between launches
+  uint32_t *cnt;   // [3 W], zero between launches: by slot of a join's first part, then by first workgroup of a group
   int W;
 };
 constexpr int kDecRows = 32;  // query rows of a block at most (the partial slots' size)

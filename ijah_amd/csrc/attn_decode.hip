@@ -27,6 +27,8 @@ namespace ijah {
 
 namespace {
 
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
 constexpr float kNegInf = -__builtin_inff();
 
 // waves of a workgroup: with 256 dims a wave's keys, values and sums take more than the 256 registers of eight waves
@@ -75,12 +77,20 @@ __device__ __forceinline__ u32x4 part_of(f32x8 &x) {
   return w;
 }
 
+// 16 bytes of a partial, device-coherent (sc1: past the XCD's own L2), by byte offset in the partials
+__device__ __forceinline__ f32x4 part_load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 16));
+}
+__device__ __forceinline__ void part_store(__amdgpu_buffer_rsrc_t r, uint32_t at, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, (int)at, 0, 16);
+}
+
 // the batch's place where a workgroup's share begins, and its walk from group to group
 struct Group {
-  int b, h, rb;      // sequence, key head, block of query rows
+  int b, h, rb;  // sequence, key head, block of query rows
   KvSeq q;
   DecSeq d;
-  int64_t u0;        // the group's first unit
+  int u0;        // the group's first unit
 };
 
 template <int KIND, int D, int RT>
@@ -90,55 +100,77 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
   constexpr int KG = KIND == kKvI8 ? KC / 2 : KC;  // granules of 16 keys
   constexpr int DB = D / 16;
   constexpr int VG = KIND == kKvI8 ? 1 : 2;        // granules of 16 dims
-  constexpr int BLK = kv_block_bytes(KIND, D);
+  constexpr int BLK = kv_block_bytes(KIND, D), SLOT = dec_slot_floats(D);
   constexpr bool F16 = KIND != kKvBf16;
   constexpr float kLift = F16 ? 14.f : 0.f;
-  // LDS: the query parts [NS][RT][KC][64 lanes] granules; for the join the waves' sums [NW][BR][kJ + 4], in turns of kJ dims
-  constexpr int kJ = 32;
-  constexpr int kQBytes = NS * RT * KC * 1024, kJBytes = NW * BR * (kJ + 4) * 4;
+  constexpr bool kAhead = RT == 1;  // the next page's keys are requested a page ahead (two row tiles leave no registers)
+  constexpr int kPitch = D + 4;     // of a row of sums in LDS
+  // LDS: the query parts [NS][RT][KC][64 lanes] granules, then the waves' sums [NW][BR][kPitch] for their join
   extern __shared__ __align__(16) uint8_t lds[];
   u32x4 *qf = (u32x4 *)lds;
   float *js = (float *)lds;
-  __shared__ int64_t sum[NT / 64 + 4];
-  __shared__ float wm[NW][BR], wl[NW][BR], jf[NW][BR], jl[BR], jmax[BR];
+  __shared__ int sum[NW + 2];
+  __shared__ float wm[NW][BR], wl[NW][BR], pm[kJoin][BR], pl[kJoin][BR];
   __shared__ int flag;
   __shared__ uint32_t qmax[BR];
-  static_assert(kQBytes <= 160 * 1024 && kJBytes <= 160 * 1024);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4,
             col = lane & 15;
-  const int group = a.Hq / a.H;
+  const int group = a.Hq / a.H, W = a.W, me = blockIdx.x;
   auto load_q = [&](int64_t row, int c) {
     return a.type == kRowF32    ? load8<kRowF32>(a.q, row, c)
            : a.type == kRowBf16 ? load8<kRowBf16>(a.q, row, c)
                                 : load8<kRowF16>(a.q, row, c);
   };
-  auto units = [&](int b) {
-    const DecSeq d = dec_seq(kv_seq(a.s, b), group, BR);
-    return (int64_t)d.pages * d.blocks * a.H;
-  };
-  // the share: all units first, then the place of the first (the scan again, over values that are now in the caches)
-  int64_t before = 0, all = 0;
-  find_item<NT>(a.s.n, -1, sum, &before, &all, units);
-  const int64_t share = dec_share(all, a.W, NW), u_lo = share * blockIdx.x, u_hi = min(u_lo + share, all);
-  if (u_lo >= u_hi) return;
+  // ---- the share
+  int pad = NW;
+  auto units = [&](int b) { return dec_units(dec_seq(kv_seq(a.s, b), group, BR), a.H, pad); };
+  BatchScan<NT> sc = scan_batch<NT>(a.s.n, sum, units);
+  int share = NW;
+  if (sc.total > W * NW) {
+    pad = 1;
+    sc = scan_batch<NT>(a.s.n, sum, units);
+    share = (int)(((uint32_t)sc.total + (uint32_t)W - 1) / (uint32_t)W);
+  }
+  if ((int64_t)share * me >= sc.total) return;
+  const int u_lo = share * me, u_hi = share < sc.total - u_lo ? u_lo + share : sc.total;
   Group g;
-  g.b = find_item<NT>(a.s.n, u_lo, sum, &before, &all, units);
+  int before;
+  g.b = find_item<NT>(sc, a.s.n, u_lo, sum, &before, units);
   g.q = kv_seq(a.s, g.b);
   g.d = dec_seq(g.q, group, BR);
+  int size = dec_units(g.d, 1, pad) / max(g.d.blocks, 1);  // the group's units
   {
-    const int64_t in = u_lo - before;
-    const int64_t per_head = (int64_t)g.d.pages * g.d.blocks;
-    g.h = (int)(in / per_head);
-    g.rb = (int)(in % per_head / g.d.pages);
-    g.u0 = before + g.h * per_head + (int64_t)g.rb * g.d.pages;
+    const int k = (u_lo - before) / size;
+    g.h = k / g.d.blocks;
+    g.rb = k - g.h * g.d.blocks;
+    g.u0 = before + k * size;
   }
-  int64_t u = u_lo;
+  int u = u_lo;
   for (;;) {  // one segment: the units [u, end) of group g
-    const int64_t g1 = g.u0 + g.d.pages, end = min(g1, u_hi);
-    const int pg0 = (int)(u - g.u0), pg1 = (int)(end - g.u0);
+    const int g1 = g.u0 + size, end = min(g1, u_hi);
+    const int pg0 = u - g.u0, pg1 = min(end - g.u0, (g.q.len + kKvPage - 1) / kKvPage);  // its pages (none: an empty sequence)
     const int nrows = min(g.q.nr * group - g.rb * BR, BR);
-    __syncthreads();  // the segment before has left LDS
+    const int *table = a.s.table + (int64_t)g.b * a.s.ldt;
+    const int turns = pg0 + wave < pg1 ? (pg1 - pg0 - wave + NW - 1) / NW : 0;  // of this wave, which has every NW-th page
+    // the page ids of the wave's next 64 turns, one a lane
+    auto load_ids = [&](int t) { return table[min(pg0 + wave + (t + lane) * NW, pg1 - 1)]; };
+    int ids = 0, id = 0;
+    u32x4 kf[4][KG], vf[DB][VG];
+    auto valid = [&](int i) { return i >= 0 && i < a.s.pages; };
+    auto block = [&](int i) { return a.base + ((int64_t)(valid(i) ? i : 0) * a.H + g.h) * BLK; };
+    auto load_keys = [&](int i) {
+      const u32x4 *kp = (const u32x4 *)block(i) + lane;
+#pragma unroll
+      for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+        for (int c = 0; c < KG; c++) kf[kb][c] = kp[(kb * KG + c) * 64];
+    };
+    if (turns) {
+      ids = load_ids(0);
+      id = __builtin_amdgcn_readlane(ids, 0);
+      if constexpr (kAhead) load_keys(id);
+    }
     // ---- the block's query rows, scaled, in parts: granule (part, tile, chunk, lane) = 8 dims of row `col`
     constexpr int QN = (RT * KC * 64 + NT - 1) / NT;
     f32x8 x[QN];
@@ -154,6 +186,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
         for (int k = 0; k < 8; k++) x[n][k] = 0.f;
       }
     }
+    __syncthreads();  // the segment before has left LDS
     if constexpr (F16) {
       if (tid < BR) qmax[tid] = 0;
       __syncthreads();
@@ -193,7 +226,6 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
       seen[t] = t * 16 + col < nrows ? g.q.len - g.q.nr + row / group : -1;
     }
     const int all_see = g.q.len - g.q.nr + g.rb * BR / group;  // every row of the block sees up to here
-    __syncthreads();
     f32x4 o[RT][DB];
     float mx[RT], l[RT];
     int ve = -200;  // 8 bits: the power of two that the sums are in units of (below any step's)
@@ -204,25 +236,20 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
 #pragma unroll
       for (int i = 0; i < DB; i++) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int *table = a.s.table + (int64_t)g.b * a.s.ldt;
-    for (int pg = pg0 + wave; pg < pg1; pg += NW) {
-      if (pg * kKvPage >= g.q.len) break;  // an empty sequence's only unit
-      const int id = __builtin_amdgcn_readfirstlane(table[pg]);
-      if (id < 0 || id >= a.s.pages) continue;
-      const uint8_t *blk = a.base + ((int64_t)id * a.H + g.h) * BLK;
-      const u32x4 *kp = (const u32x4 *)blk + lane, *vp = (const u32x4 *)(blk + kKvPage * D * kv_esize(KIND)) + lane;
-      u32x4 kf[4][KG], vf[DB][VG];
-#pragma unroll
-      for (int kb = 0; kb < 4; kb++)
-#pragma unroll
-        for (int c = 0; c < KG; c++) kf[kb][c] = kp[(kb * KG + c) * 64];
+    __syncthreads();
+    for (int it = 0; it < turns; it++) {
+      const int pg = pg0 + wave + it * NW;
+      const uint8_t *blk = block(id);
+      const u32x4 *vp = (const u32x4 *)(blk + kKvPage * D * kv_esize(KIND)) + lane;
+      const bool there = valid(id);  // a page id outside the pool: a page that nobody sees
+      const int len = there ? g.q.len : 0;
+      if constexpr (!kAhead) load_keys(id);
       auto load_values = [&] {
 #pragma unroll
         for (int i = 0; i < DB; i++)
 #pragma unroll
           for (int v = 0; v < VG; v++) vf[i][v] = vp[(i * VG + v) * 64];
       };
-      if constexpr (RT == 1) load_values();
       f32x4 ks[4], vs[4];
       auto load_steps = [&] {
 #pragma unroll
@@ -231,8 +258,11 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
           vs[kb] = *(const f32x4 *)(blk + kv_step_at(D, 1, kb * 16 + quad * 4));
         }
       };
-      if constexpr (KIND == kKvI8 && RT == 1) load_steps();
-      const bool edge = pg * kKvPage + kKvPage - 1 > all_see;  // some row does not see some key of the page
+      if constexpr (kAhead) {
+        load_values();
+        if constexpr (KIND == kKvI8) load_steps();
+      }
+      const bool edge = pg * kKvPage + kKvPage - 1 > all_see || !there;  // some row does not see some key of the page
       const int j0 = pg * kKvPage + quad * 4;
       // ---- scores: lane (row col, keys kb * 16 + 4 quad + i)
       f32x4 s[RT][4];
@@ -261,15 +291,28 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
             }
           }
       }
+      if constexpr (kAhead) {
+        if (it + 1 < turns) {
+          if (((it + 1) & 63) == 0) ids = load_ids(it + 1);
+          id = __builtin_amdgcn_readlane(ids, (it + 1) & 63);
+          load_keys(id);
+        }
+      } else {
+        load_values();
+        if constexpr (KIND == kKvI8) load_steps();
+        if (it + 1 < turns) {
+          if (((it + 1) & 63) == 0) ids = load_ids(it + 1);
+          id = __builtin_amdgcn_readlane(ids, (it + 1) & 63);
+        }
+      }
       float vshift = 1.f;
-      if constexpr (KIND == kKvI8 && RT > 1) load_steps();
       if constexpr (KIND == kKvI8) {
         float top = 0.f;
 #pragma unroll
         for (int kb = 0; kb < 4; kb++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            if (edge && j0 + kb * 16 + i >= g.q.len) vs[kb][i] = 0.f;  // behind the last token a step may be anything
+            if (edge && j0 + kb * 16 + i >= len) vs[kb][i] = 0.f;  // behind the last token a step may be anything
             top = fmaxf(top, vs[kb][i]);
           }
         top = fmaxf(top, xor_lane<16>(top, lane));
@@ -283,10 +326,10 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
           for (int i = 0; i < 4; i++) vs[kb][i] = __builtin_amdgcn_ldexpf(vs[kb][i], -e);
         }
       }
-      if constexpr (RT > 1) load_values();  // (two row tiles leave no registers for both)
       f32x8 p[RT][2];
 #pragma unroll
       for (int t = 0; t < RT; t++) {
+        const int last = there ? seen[t] : -1;
         float top = kNegInf;
 #pragma unroll
         for (int kb = 0; kb < 4; kb++)
@@ -294,7 +337,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
           for (int i = 0; i < 4; i++) {
             float v = s[t][kb][i] * scale[t];
             if constexpr (KIND == kKvI8) v *= ks[kb][i];
-            if (edge) v = j0 + kb * 16 + i <= seen[t] ? v : kNegInf;
+            if (edge) v = j0 + kb * 16 + i <= last ? v : kNegInf;
             s[t][kb][i] = v;
             top = fmaxf(top, v);
           }
@@ -312,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
             add += e;
             if constexpr (KIND == kKvI8) {
               e *= vs[kb][i];
-              if (edge) e = j0 + kb * 16 + i <= seen[t] ? e : 0.f;  // (a step may be NaN)
+              if (edge) e = j0 + kb * 16 + i <= last ? e : 0.f;  // (a step may be NaN)
             }
             p[t][kb >> 1][(kb & 1) * 4 + i] = e;
           }
@@ -325,7 +368,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
       // the rows that see it are made NaN (which of them, the same product of ones tells).
       bool odd = false;
       auto kept = [&](u32x4 w, int kg) {  // the keys before len (recomputed where it is used: edges are rare, registers are not)
-        const int left = again(g.q.len - j0) - kg * 32;
+        const int left = again(len - j0) - kg * 32;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const int j = (k >> 1) * 16 + (k & 1) * 2;
@@ -408,7 +451,8 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
           for (int k = 0; k < 4; k++) o[t][i][k] = __builtin_amdgcn_ldexpf(o[t][i][k], ve);
     }
     // ---- the segment's waves joined
-    const int used = min(NW, pg1 - pg0);  // waves that had a page
+    const int used = max(min(NW, pg1 - pg0), 1);  // waves that had a page; one has the zeros of an empty sequence
+    __syncthreads();  // every wave has read its query parts
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       float s = l[t];
@@ -418,76 +462,116 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
         wm[wave][t * 16 + col] = mx[t];
         wl[wave][t * 16 + col] = s;
       }
-    }
-    __syncthreads();  // and every wave has read its query parts
-    const DecPart part = dec_part(g.u0, g1, share, (int)blockIdx.x);
-    float *slot = a.part + (int64_t)part.slot * dec_slot_floats(D);
-    if (tid < BR) {
-      float m = kNegInf, s = 0.f;
-      for (int w = 0; w < used; w++) m = fmaxf(m, wm[w][tid]);
-      const float ms = m == kNegInf ? 0.f : m;
-      for (int w = 0; w < used; w++) {
-        const float f = __builtin_amdgcn_exp2f(wm[w][tid] - ms);
-        jf[w][tid] = f;
-        s += wl[w][tid] * f;
-      }
-      jl[tid] = s == 0.f ? 0.f : 1.f / s;
-      if (part.parts > 1) {
-        st_cg(slot + BR * D + tid, m);
-        st_cg(slot + BR * D + BR + tid, s);
+      if (wave < used && t * 16 + col < nrows) {
+#pragma unroll
+        for (int i = 0; i < DB; i++) *(f32x4 *)(js + (wave * BR + t * 16 + col) * kPitch + i * 16 + quad * 4) = o[t][i];
       }
     }
-    auto out_at = [&](int m, int d, float v) {  // one output element
+    __syncthreads();
+    const DecPart part = dec_part(g.u0, g1, share, me);
+    const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)(2u * W * SLOT * 4), 0x00020000);
+    auto out4 = [&](int m, int d, f32x4 v) {  // four output elements
       const int row = g.rb * BR + m, t = row / group;
-      store1(a.out, a.type, g.q.r0 + t, (g.h * group + row - t * group) * D + d, v);
+      const int64_t at = (g.q.r0 + t) * a.out.ld + (g.h * group + row - t * group) * D + d;
+      if (a.type == kRowF32) {
+        *(f32x4 *)((float *)a.out.p + at) = v;
+      } else {
+        u32x2 w;
+        if (a.type == kRowBf16) {
+          bf16x4 o4;
+#pragma unroll
+          for (int k = 0; k < 4; k++) o4[k] = (__bf16)v[k];
+          w = __builtin_bit_cast(u32x2, o4);
+        } else {
+          f16x4 o4;
+#pragma unroll
+          for (int k = 0; k < 4; k++) o4[k] = (_Float16)v[k];
+          w = __builtin_bit_cast(u32x2, o4);
+        }
+        *(u32x2 *)((uint16_t *)a.out.p + at) = w;
+      }
     };
-#pragma unroll
-    for (int c = 0; c < D / kJ; c++) {
-      if (c) __syncthreads();
-#pragma unroll
-      for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int i = 0; i < kJ / 16; i++)
-          *(f32x4 *)(js + (wave * BR + t * 16 + col) * (kJ + 4) + i * 16 + quad * 4) = o[t][c * (kJ / 16) + i];
-      __syncthreads();
-      for (int i = tid; i < BR * kJ; i += NT) {
-        const int m = i / kJ, d = i % kJ;
-        if (m >= nrows) break;
-        float s = 0.f;
-        for (int w = 0; w < used; w++) s = __builtin_fmaf(js[(w * BR + m) * (kJ + 4) + d], jf[w][m], s);
-        if (part.parts > 1) st_cg(slot + m * D + c * kJ + d, s);
-        else out_at(m, c * kJ + d, s * jl[m]);
+    for (int i = tid; i < nrows * (D / 4); i += NT) {
+      const int m = i / (D / 4), d = i % (D / 4) * 4;
+      float top = kNegInf, s = 0.f;
+      for (int w = 0; w < used; w++) top = fmaxf(top, wm[w][m]);
+      const float ms = top == kNegInf ? 0.f : top;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < used; w++) {
+        const float f = __builtin_amdgcn_exp2f(wm[w][m] - ms);
+        s = __builtin_fmaf(wl[w][m], f, s);
+        v += *(const f32x4 *)(js + (w * BR + m) * kPitch + d) * f;
+      }
+      if (part.parts > 1) {
+        part_store(parts, (uint32_t)(part.slot * SLOT + m * D + d) * 4u, v);
+        if (d == 0) {
+          st_cg(a.part + (int64_t)part.slot * SLOT + BR * D + m, top);
+          st_cg(a.part + (int64_t)part.slot * SLOT + BR * D + BR + m, s);
+        }
+      } else {
+        out4(m, d, v * (s == 0.f ? 0.f : 1.f / s));
       }
     }
-    // ---- the group's shares joined
+    // ---- the group's shares joined: parts by kJoin, then their joins
     if (part.parts > 1) {
-      __builtin_amdgcn_s_waitcnt(0);  // this wave's partials have arrived
-      __syncthreads();
-      if (tid == 0) flag = (int)atomicAdd(a.cnt + part.first, 1u);
-      __syncthreads();
-      if (flag == part.parts - 1) {
-        const float *base = a.part + (int64_t)part.first * 2 * dec_slot_floats(D);
-        // the first share's slot is its second if the group begins inside it; the others' their first
-        auto at = [&](int k) { return base + (int64_t)(2 * k + (k == 0 && g.u0 % share != 0 ? 1 : 0)) * dec_slot_floats(D); };
-        if (tid < nrows) {
-          float m = kNegInf;
-          for (int k = 0; k < part.parts; k++) m = fmaxf(m, ld_cg(at(k) + BR * D + tid));
-          const float ms = m == kNegInf ? 0.f : m;
-          float s = 0.f;
-          for (int k = 0; k < part.parts; k++)
-            s = __builtin_fmaf(ld_cg(at(k) + BR * D + BR + tid), __builtin_amdgcn_exp2f(ld_cg(at(k) + BR * D + tid) - ms), s);
-          jmax[tid] = ms;
-          jl[tid] = s == 0.f ? 0.f : 1.f / s;
+      // parts k0, k0 + step, .. (cnt of them) into part k0's slot, or into the output
+      auto join = [&](int k0, int step, int cnt, bool final) {
+        for (int i = tid; i < cnt * BR; i += NT) {
+          const int k = i / BR, m = i % BR;
+          if (m < nrows) {
+            const float *sl = a.part + (int64_t)dec_slot(part, g.u0, share, k0 + k * step) * SLOT + BR * D;
+            pm[k][m] = ld_cg(sl + m);
+            pl[k][m] = ld_cg(sl + BR + m);
+          }
         }
         __syncthreads();
-        for (int i = tid; i < nrows * D; i += NT) {
-          const int m = i / D, d = i % D;
-          float s = 0.f;
-          for (int k = 0; k < part.parts; k++)
-            s = __builtin_fmaf(ld_cg(at(k) + m * D + d), __builtin_amdgcn_exp2f(ld_cg(at(k) + BR * D + m) - jmax[m]), s);
-          out_at(m, d, s * jl[m]);
+        for (int i = tid; i < nrows * (D / 4); i += NT) {
+          const int m = i / (D / 4), d = i % (D / 4) * 4;
+          f32x4 v = {0.f, 0.f, 0.f, 0.f}, in[kJoin];
+#pragma unroll
+          for (int k = 0; k < kJoin; k++)  // all requested at once; behind the last the first again, times 0
+            in[k] = part_load(parts, (uint32_t)(dec_slot(part, g.u0, share, k0 + (k < cnt ? k : 0) * step) * SLOT + m * D + d) * 4u);
+          float top = kNegInf, s = 0.f;
+          for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][m]);
+          const float ms = top == kNegInf ? 0.f : top;
+#pragma unroll
+          for (int k = 0; k < kJoin; k++) {
+            if (k < cnt) {
+              const float f = __builtin_amdgcn_exp2f(pm[k][m] - ms);
+              s = __builtin_fmaf(pl[k][m], f, s);
+              v += in[k] * f;
+            }
+          }
+          if (final) {
+            out4(m, d, v * (s == 0.f ? 0.f : 1.f / s));
+          } else {
+            const int to = dec_slot(part, g.u0, share, k0) * SLOT;
+            part_store(parts, (uint32_t)(to + m * D + d) * 4u, v);
+            if (d == 0) {
+              st_cg(a.part + to + BR * D + m, top);
+              st_cg(a.part + to + BR * D + BR + m, s);
+            }
+          }
         }
-        if (tid == 0) st_cg(a.cnt + part.first, 0u);
+      };
+      auto last_of = [&](uint32_t *c, int n) {  // every wave's stores have arrived; true in the n-th workgroup to come here
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (tid == 0) {
+          flag = atomicAdd(c, 1u) == (uint32_t)n - 1u;
+          if (flag) st_cg(c, 0u);
+        }
+        __syncthreads();
+        return flag != 0;
+      };
+      const int k = me - part.first, k0 = k / kJoin * kJoin, cnt = min(part.parts - k0, kJoin);
+      const bool one = part.parts <= kJoin;
+      if (cnt == 1 || last_of(a.cnt + dec_slot(part, g.u0, share, k0), cnt)) {
+        if (cnt > 1) join(k0, 1, cnt, one);
+        if (!one) {
+          const int joins = (part.parts + kJoin - 1) / kJoin;  // at most kJoin: W <= kJoin^2
+          if (last_of(a.cnt + 2 * W + part.first, joins)) join(0, kJoin, joins, true);
+        }
       }
     }
     if (end == u_hi) return;
@@ -499,10 +583,11 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
       if (++g.h == a.H) {
         g.h = 0;
         do {
-          if (++g.b >= a.s.n) return;  // (not reached: u < all, so a later sequence has rows)
+          if (++g.b >= a.s.n) return;  // (not reached: u < total, so a later sequence has rows)
           g.q = kv_seq(a.s, g.b);
           g.d = dec_seq(g.q, group, BR);
         } while (!g.d.blocks);
+        size = dec_units(g.d, 1, pad) / g.d.blocks;
       }
     }
   }
@@ -510,7 +595,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
 
 template <int KIND, int D, int RT>
 constexpr int lds_bytes() {
-  constexpr int q = Num<KIND>::NS * RT * (D / 32) * 1024, j = kWaves<D> * 16 * RT * 36 * 4;
+  constexpr int q = Num<KIND>::NS * RT * (D / 32) * 1024, j = kWaves<D> * 16 * RT * (D + 4) * 4;
   return q > j ? q : j;
 }
 
@@ -536,7 +621,7 @@ int decode_grid() {
   int dev = 0, cus = 0;
   IJ_HIP(hipGetDevice(&dev));
   IJ_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-  return cus;
+  return std::min(cus, kJoin * kJoin);  // (256 on an MI355X) joins of joins are one level
 }
 
 void launch_attn_decode(const DecArgs &a, hipStream_t s) {

@@ -87,47 +87,76 @@ __device__ __forceinline__ f16x8 i8_f16(u32x2 w) {
   return h;
 }
 
-// ---- the sequence in which item `item` of a batch lies, items(b) each: every thread of the workgroup (NT threads)
-// calls this; sum: [NT / 64 + 4] words of LDS. Returns the sequence, or -1 behind the last; *before = items of the
-// sequences before it, *all = of the whole batch. The sequences are divided among the threads in order, one scan over
-// the threads' sums, then the thread whose range holds the item walks it.
+// ---- division of a batch: which sequence the item `item` lies in, with items(b) of each sequence b (32-bit totals: the
+// host refuses more). Up to 256 sequences every wave scans the batch on its own, with neither LDS nor a barrier: a lane sums
+// its next ceil(n / 64), one scan over the lanes, and the lane whose range holds the item walks it. More sequences are
+// divided among all threads of the workgroup.
+__device__ __forceinline__ int wave_scan(int x) {  // inclusive sum over the lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // a row's last lane to the next row's: rows 1, 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31 to rows 2, 3
+  return x;
+}
+constexpr int kWaveScan = 256;
+template <int NT>
+struct BatchScan {
+  int b0, b1, at, mine, total;  // this thread's sequences, the items before them, of them, of the batch
+};
+// sum: [NT / 64 + 2] words of LDS, the workgroup's from here until the last find
 template <int NT, typename F>
-__device__ int find_item(int n, int64_t item, int64_t *sum, int64_t *before, int64_t *all, F &&items) {
-  const int tid = threadIdx.x, per = (n + NT - 1) / NT, lane = tid & 63;
-  const int b0 = min(tid * per, n), b1 = min(b0 + per, n);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; b++) mine += items(b);
-  int64_t inc = mine;  // inclusive scan within the wave
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t up = __shfl_up(inc, d);
-    if (lane >= d) inc += up;
+__device__ __forceinline__ BatchScan<NT> scan_batch(int n, int *sum, F &&items) {
+  BatchScan<NT> s;
+  const bool wide = n > kWaveScan;
+  const int t = wide ? threadIdx.x : threadIdx.x & 63, per = wide ? (n + NT - 1) / NT : (n + 63) >> 6;
+  s.b0 = min(t * per, n);
+  s.b1 = min(s.b0 + per, n);
+  s.mine = 0;
+  for (int b = s.b0; b < s.b1; b++) s.mine += items(b);
+  const int inc = wave_scan(s.mine);
+  s.at = inc - s.mine;
+  s.total = __builtin_amdgcn_readlane(inc, 63);
+  if (wide) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sum[threadIdx.x >> 6] = inc;
+    __syncthreads();
+    s.total = 0;
+    for (int w = 0; w < NT / 64; w++) {
+      if (w < (int)(threadIdx.x >> 6)) s.at += sum[w];
+      s.total += sum[w];
+    }
   }
-  __syncthreads();
-  if (lane == 63) sum[tid >> 6] = inc;
-  if (tid == 0) sum[NT / 64] = -1;
-  __syncthreads();
-  int64_t base = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; w++) {
-    if (w < (tid >> 6)) base += sum[w];
-    total += sum[w];
-  }
-  *all = total;
-  int64_t at = base + inc - mine;
-  if (item >= at && item < at + mine) {
-    int b = b0;
+  return s;
+}
+// the sequence of item `item` (uniform, < total), *before = the items of the sequences before it
+template <int NT, typename F>
+__device__ __forceinline__ int find_item(const BatchScan<NT> &s, int n, int item, int *sum, int *before, F &&items) {
+  const bool mine = item >= s.at && item < s.at + s.mine;
+  int b = s.b0, at = s.at;
+  if (mine) {
     for (;; b++) {
-      const int64_t k = items(b);
-      if (item < at + k) break;
+      const int k = items(b);
+      if (item < at + k || b + 1 >= s.b1) break;
       at += k;
     }
-    sum[NT / 64] = b;
-    sum[NT / 64 + 1] = at;
   }
-  __syncthreads();
-  *before = sum[NT / 64 + 1];
-  return (int)sum[NT / 64];
+  if (n > kWaveScan) {
+    if (mine) {
+      sum[NT / 64] = b;
+      sum[NT / 64 + 1] = at;
+    }
+    __syncthreads();
+    b = sum[NT / 64];
+    at = sum[NT / 64 + 1];
+  } else {
+    const int lane = (int)__builtin_ctzll(__ballot(mine) | 1ull << 63);
+    b = __builtin_amdgcn_readlane(b, lane);
+    at = __builtin_amdgcn_readlane(at, lane);
+  }
+  *before = __builtin_amdgcn_readfirstlane(at);
+  return __builtin_amdgcn_readfirstlane(b);
 }
 
 }  // namespace ijah

@@ -17,7 +17,7 @@ struct ne_kv {
   uint64_t layer_bytes = 0;
   uint8_t *base = nullptr;
   float *part = nullptr;    // decode: the partial slots of W workgroups
-  uint32_t *cnt = nullptr;  // decode: W counters, zero between launches
+  uint32_t *cnt = nullptr;  // decode: 3 W counters, zero between launches
   ~ne_kv() {
     for (void *p : {(void *)base, (void *)part, (void *)cnt})
       if (p) (void)hipFree(p);
@@ -159,7 +159,7 @@ NE_API ne_kv *ne_kv_create(const ne_kv_desc *d) {
     kv->layer_bytes = per_page * (uint64_t)d->pages;
     alloc(kv->base, kv->layer_bytes * (uint64_t)d->layers);
     alloc(kv->part, (uint64_t)2 * kv->W * dec_slot_floats(d->dim) * 4);
-    alloc(kv->cnt, (uint64_t)kv->W * 4);
+    alloc(kv->cnt, (uint64_t)3 * kv->W * 4);
     IJ_HIP(hipDeviceSynchronize());
     h = kv.release();
   });
@@ -201,7 +201,9 @@ NE_API int ne_attn_decode(ne_kv *kv, int layer, const ne_kv_seqs *s, int R, int 
     check_scale(scale);
     DecArgs a;
     a.s = seqs_of(kv, s, R);
-    IJ_CHECK((int64_t)R * heads <= std::numeric_limits<int>::max(), "%d rows of %d heads", R, heads);
+    IJ_CHECK(dec_max_units(s->n, s->ldt, R, heads / kv->d.heads, kv->d.heads, 16, 8) < (1ll << 31) &&
+                 (int64_t)R * heads < (1ll << 31),
+             "%d rows of %d heads over %d tables of %d pages: too much for one call", R, heads, s->n, s->ldt);
     a.kind = kv->kind;
     a.D = kv->d.dim;
     a.H = kv->d.heads;

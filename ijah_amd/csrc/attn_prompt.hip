@@ -59,20 +59,20 @@ template <int D, int BN, int NT, bool F16>
 __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
   constexpr int KC = D / 16, DB = D / 32, KB = BN / 32, CH = D / 8, kPlane = BN * D * 2;
   extern __shared__ __align__(16) uint8_t lds[];  // keys [NT][BN][D], values [NT][BN][D]
-  __shared__ int64_t sum[8];
+  __shared__ int sum[6];
   __shared__ uint32_t odd[BN];  // keys of the tile whose value is not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5,
             col = lane & 31;
   auto bound = [](const int *p, int b, int R) { return kv_clamp(p[b], 0, R); };
   auto q_of = [&](int b) { return max(bound(a.q_rows, b + 1, a.Rq) - bound(a.q_rows, b, a.Rq), 0); };
-  int64_t before = 0, all = 0;
   // the last blocks see the most keys: they go first
-  const int64_t blocks = gridDim.x / a.Hq;
-  const int h = blockIdx.x % a.Hq;
-  const int64_t item = blocks - 1 - blockIdx.x / a.Hq;
-  const int b = find_item<256>(a.n, item, sum, &before, &all, [&](int i) { return (int64_t)((q_of(i) + kBM - 1) / kBM); });
-  if (b < 0) return;
-  const int nq = q_of(b), q0 = bound(a.q_rows, b, a.Rq), i0 = (int)(item - before) * kBM;
+  const int blocks = gridDim.x / a.Hq, h = blockIdx.x % a.Hq, item = blocks - 1 - (int)blockIdx.x / a.Hq;
+  auto items = [&](int i) { return (q_of(i) + kBM - 1) / kBM; };
+  const BatchScan<256> sc = scan_batch<256>(a.n, sum, items);
+  if (item >= sc.total) return;
+  int before;
+  const int b = find_item<256>(sc, a.n, item, sum, &before, items);
+  const int nq = q_of(b), q0 = bound(a.q_rows, b, a.Rq), i0 = (item - before) * kBM;
   const int k0 = bound(a.k_rows, b, a.Rk), nk = max(bound(a.k_rows, b + 1, a.Rk) - k0, 0);
   const int off = nk - nq, hk = h / (a.Hq / a.H);
   const int row = i0 + wave * 32 + col;  // this lane's query row in its sequence

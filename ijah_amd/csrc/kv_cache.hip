@@ -31,20 +31,18 @@ struct Piece {
 
 // the workgroup's piece; false behind the last
 template <int NT>
-__device__ bool find_piece(const KvSeqs &s, int64_t item, int64_t *sum, Piece *p) {
-  int64_t before = 0, all = 0;
-  int b;
+__device__ __forceinline__ bool find_piece(const KvSeqs &s, int item, int *sum, Piece *p) {
+  int before = item, b = item;
   if (s.rows) {
-    b = find_item<NT>(s.n, item, sum, &before, &all, [&](int i) { return (int64_t)kv_pieces(kv_seq(s, i)); });
-    if (b < 0) return false;
-  } else {
-    b = (int)item;
-    before = item;
+    auto items = [&](int i) { return kv_pieces(kv_seq(s, i)); };
+    const BatchScan<NT> sc = scan_batch<NT>(s.n, sum, items);
+    if (item >= sc.total) return false;
+    b = find_item<NT>(sc, s.n, item, sum, &before, items);
   }
   const KvSeq q = kv_seq(s, b);
   if (!q.nr) return false;
   const int first = q.len - q.nr, p0 = max(first, 0);  // the first row's token; the first token written
-  const int k = (int)(item - before), pg = p0 / kKvPage + k;
+  const int k = item - before, pg = p0 / kKvPage + k;
   p->b = b;
   p->nr_before = k == 0 ? p0 - first : 0;
   p->lead0 = q.r0;
@@ -62,12 +60,12 @@ __device__ bool find_piece(const KvSeqs &s, int64_t item, int64_t *sum, Piece *p
 template <int KIND, int D, int TYPE>
 __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
   constexpr int NT = kThreads<D>, kPitch = D * kv_esize(KIND) + 4;  // bytes of a tile row in LDS
-  __shared__ int64_t sum[NT / 64 + 4];
+  __shared__ int sum[NT / 64 + 2];
   __shared__ uint32_t amax[2][NT / 64][16];
   __shared__ __align__(16) uint8_t tile[kKvPage * kPitch];
   const int tid = threadIdx.x, tok = tid & 15, part = tid >> 4, h = blockIdx.y;
   Piece p;
-  if (!find_piece<NT>(a.s, blockIdx.x, sum, &p) || p.page < 0) return;
+  if (!find_piece<NT>(a.s, (int)blockIdx.x, sum, &p) || p.page < 0) return;
   uint8_t *blk = a.base + ((int64_t)p.page * a.H + h) * kv_block_bytes(KIND, D);
   for (int g = p.j0 >> 4; g <= (p.j1 - 1) >> 4; g++) {
     const int j = g * 16 + tok;
@@ -185,11 +183,11 @@ __device__ __forceinline__ f32x8 widen8(u32x2 w, float s) {
 template <int KIND, int D, int TYPE>
 __global__ __launch_bounds__(kThreads<D>) void kv_read(KvArgs a) {
   constexpr int NT = kThreads<D>, E = kv_esize(KIND), kPitch = D * E + 4;
-  __shared__ int64_t sum[NT / 64 + 4];
+  __shared__ int sum[NT / 64 + 2];
   __shared__ __align__(16) uint8_t tile[kKvPage * kPitch];
   const int tid = threadIdx.x, tok = tid & 15, part = tid >> 4, h = blockIdx.y;
   Piece p;
-  if (!find_piece<NT>(a.s, blockIdx.x, sum, &p)) return;
+  if (!find_piece<NT>(a.s, (int)blockIdx.x, sum, &p)) return;
   const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int i = tok; i < p.nr_before; i += 16) {
     store8<TYPE>(a.k, p.lead0 + i, h * D + part * 8, zero);

@@ -15,7 +15,6 @@ ROOT = Path(__file__).resolve().parents[1]
 PROGRAM = r"""
 #include <cstdio>
 #include <cstdlib>
-#include <map>
 #include <random>
 #include <set>
 #include <vector>
@@ -85,39 +84,54 @@ static void pieces(std::mt19937 &r) {
 static void shares(std::mt19937 &r) {
   for (int it = 0; it < 3000; it++) {
     Batch b = batch(r, 1 + r() % 30, 1 + r() % (it % 5 ? 900 : 60000), 1 + r() % 8, it % 2);
-    const int W = 1 + r() % 300, H = 1 + r() % 8, group = 1 + r() % 20, BR = r() % 2 ? 16 : 32, least = r() % 2 ? 4 : 8;
-    std::vector<std::pair<int64_t, int64_t>> groups;
-    int64_t all = 0;
-    for (int i = 0; i < b.s.n; i++) {
-      const DecSeq d = dec_seq(kv_seq(b.s, i), group, BR);
-      CHECK(d.pages >= 1 && d.blocks >= 0);
-      for (int k = 0; k < H * d.blocks; k++, all += d.pages) groups.push_back({all, all + d.pages});
+    const int W = 1 + r() % 256, H = 1 + r() % 8, group = 1 + r() % 20, BR = r() % 2 ? 16 : 32, least = r() % 2 ? 4 : 8;
+    // the two forms, as the kernel chooses them
+    auto total = [&](int pad) {
+      int t = 0;
+      for (int i = 0; i < b.s.n; i++) t += dec_units(dec_seq(kv_seq(b.s, i), group, BR), H, pad);
+      CHECK(t <= dec_max_units(b.s.n, b.s.ldt, b.s.R, group, H, 16, 8));
+      return t;
+    };
+    int pad = least, all = total(pad), share = least;
+    if (all > W * least) {
+      pad = 1;
+      all = total(pad);
+      share = (all + W - 1) / W;
     }
     if (!all) continue;
-    const int64_t share = dec_share(all, W, least);
-    CHECK(share * W >= all && share >= least);
-    std::set<int> slots, counters;
-    std::map<int64_t, int> covered;  // units of each group seen
+    CHECK((int64_t)share * W >= all);
+    std::set<int> slots, counters, firsts;
     int64_t units = 0;
-    for (auto g : groups) {
-      const int first = (int)(g.first / share), last = (int)((g.second - 1) / share);
-      CHECK(last < W);
-      for (int w = first; w <= last; w++) {
-        const int64_t lo = std::max(g.first, share * w), hi = std::min(g.second, share * (w + 1));
-        CHECK(lo < hi);
-        units += hi - lo;
-        const DecPart p = dec_part(g.first, g.second, share, w);
-        CHECK(p.first == first && p.parts == last - first + 1);
-        if (p.parts > 1) {
-          CHECK(p.slot >= 0 && p.slot < 2 * W && slots.insert(p.slot).second);
-          // where the join looks for part k = w - first
-          const int k = w - first;
-          CHECK(p.slot == 2 * first + 2 * k + (k == 0 && g.first % share != 0 ? 1 : 0));
+    int at = 0;
+    for (int i = 0; i < b.s.n; i++) {
+      const KvSeq q = kv_seq(b.s, i);
+      const DecSeq d = dec_seq(q, group, BR);
+      CHECK(d.pages >= 1 && d.blocks >= 0);
+      for (int k = 0; k < H * d.blocks; k++) {
+        const int g0 = at, g1 = g0 + dec_units(d, 1, pad) / d.blocks, first = g0 / share, last = (g1 - 1) / share;
+        at = g1;
+        CHECK(last < W);
+        int real = 0;
+        for (int w = first; w <= last; w++) {
+          const int lo = std::max(g0, share * w), hi = std::min(g1, share * (w + 1));
+          CHECK(lo < hi);
+          const int p0 = lo - g0, p1 = std::min(hi - g0, (q.len + kKvPage - 1) / kKvPage);
+          CHECK(p0 < p1 || (q.len == 0 && p0 == 0));
+          real += std::max(p1 - p0, 0);
+          const DecPart p = dec_part(g0, g1, share, w);
+          CHECK(p.first == first && p.parts == last - first + 1 && p.parts <= kJoin * kJoin);
+          if (p.parts > 1) {
+            CHECK(p.slot >= 0 && p.slot < 2 * W && slots.insert(p.slot).second);
+            CHECK(p.slot == dec_slot(p, g0, share, w - first));
+            if ((w - first) % kJoin == 0) CHECK(counters.insert(p.slot).second);
+          }
         }
+        CHECK(real == (q.len + kKvPage - 1) / kKvPage);
+        units += g1 - g0;
+        if (last > first) CHECK(firsts.insert(first).second);
       }
-      if (last > first) CHECK(counters.insert(first).second);
     }
-    CHECK(units == all);
+    CHECK(units == all && at == all);
   }
 }
 int main() {
