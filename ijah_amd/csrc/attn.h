@@ -109,7 +109,7 @@ IJ_HD int dec_units(const DecSeq &d, int H, int pad) { return (d.pages + pad - 1
 IJ_HD int64_t dec_max_units(int n, int ldt, int R, int group, int H, int block_rows, int pad) {
   return ((int64_t)R * group / block_rows + n) * H * ((int64_t)ldt + pad);
 }
-constexpr int kJoin = 16;
+constexpr int kJoin = 16, kJoins = 32;  // parts of a join, joins of a join of joins: W <= kJoin kJoins
 struct DecPart {
   int first, parts, slot;  // the group's first workgroup, how many it has, this one's partial slot
 };
@@ -160,7 +160,7 @@ struct PromptArgs {
 };
 void launch_kv_write(const KvArgs &a, hipStream_t s);
 void launch_kv_read(const KvArgs &a, hipStream_t s);
-int decode_grid();  // workgroups of the decode kernel: one per CU
+int decode_grid(int D);  // workgroups of the decode kernel: what the chip runs at once
 void launch_attn_decode(const DecArgs &a, hipStream_t s);
 void launch_attn_prompt(const PromptArgs &a, hipStream_t s);
 void init_attn_attrs();  // raises the kernels' dynamic LDS limits: before any launch and outside a capture

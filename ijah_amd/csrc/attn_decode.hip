@@ -31,9 +31,10 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
 
-// waves of a workgroup: with 256 dims a wave's keys, values and sums take more than the 256 registers of eight waves
-template <int D>
-constexpr int kWaves = D == 256 ? 4 : 8;
+// A workgroup has four waves; with up to 128 dims two of them share a CU (256 registers a wave), so that one's joins and
+// first requests pass under the other's pages. With 256 dims a wave's keys, values and sums take up to 512 registers.
+constexpr int NW = 4, NT = 64 * NW;
+IJ_HD constexpr int per_cu(int D) { return D == 256 ? 1 : 2; }
 
 template <int KIND>
 struct Num {  // the matrix type of a cache kind, and the parts an f32 operand is cut into
@@ -94,8 +95,8 @@ struct Group {
 };
 
 template <int KIND, int D, int RT>
-__global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
-  constexpr int NW = kWaves<D>, NT = 64 * NW, NS = Num<KIND>::NS, BR = 16 * RT;
+__global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
+  constexpr int NS = Num<KIND>::NS, BR = 16 * RT;
   constexpr int KC = D / 32;                       // products of 32 dims
   constexpr int KG = KIND == kKvI8 ? KC / 2 : KC;  // granules of 16 keys
   constexpr int DB = D / 16;
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
   u32x4 *qf = (u32x4 *)lds;
   float *js = (float *)lds;
   __shared__ int sum[NW + 2];
-  __shared__ float wm[NW][BR], wl[NW][BR], pm[kJoin][BR], pl[kJoin][BR];
+  __shared__ float wm[NW][BR], wl[NW][BR], pm[kJoins][BR], pl[kJoins][BR];
   __shared__ int flag;
   __shared__ uint32_t qmax[BR];
 
@@ -528,18 +529,22 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
         for (int i = tid; i < nrows * (D / 4); i += NT) {
           const int m = i / (D / 4), d = i % (D / 4) * 4;
           f32x4 v = {0.f, 0.f, 0.f, 0.f}, in[kJoin];
-#pragma unroll
-          for (int k = 0; k < kJoin; k++)  // all requested at once; behind the last the first again, times 0
-            in[k] = part_load(parts, (uint32_t)(dec_slot(part, g.u0, share, k0 + (k < cnt ? k : 0) * step) * SLOT + m * D + d) * 4u);
           float top = kNegInf, s = 0.f;
-          for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][m]);
-          const float ms = top == kNegInf ? 0.f : top;
+          for (int r = 0; r < cnt; r += kJoin) {
 #pragma unroll
-          for (int k = 0; k < kJoin; k++) {
-            if (k < cnt) {
-              const float f = __builtin_amdgcn_exp2f(pm[k][m] - ms);
-              s = __builtin_fmaf(pl[k][m], f, s);
-              v += in[k] * f;
+            for (int k = 0; k < kJoin; k++)  // all requested at once; behind the last the first again, not used
+              in[k] = part_load(parts, (uint32_t)(dec_slot(part, g.u0, share, k0 + (r + k < cnt ? r + k : 0) * step) * SLOT +
+                                                  m * D + d) * 4u);
+            if (r == 0)
+              for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][m]);
+            const float ms = top == kNegInf ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < kJoin; k++) {
+              if (r + k < cnt) {
+                const float f = __builtin_amdgcn_exp2f(pm[r + k][m] - ms);
+                s = __builtin_fmaf(pl[r + k][m], f, s);
+                v += in[k] * f;
+              }
             }
           }
           if (final) {
@@ -569,7 +574,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
       if (cnt == 1 || last_of(a.cnt + dec_slot(part, g.u0, share, k0), cnt)) {
         if (cnt > 1) join(k0, 1, cnt, one);
         if (!one) {
-          const int joins = (part.parts + kJoin - 1) / kJoin;  // at most kJoin: W <= kJoin^2
+          const int joins = (part.parts + kJoin - 1) / kJoin;  // at most kJoins
           if (last_of(a.cnt + 2 * W + part.first, joins)) join(0, kJoin, joins, true);
         }
       }
@@ -595,7 +600,7 @@ __global__ __launch_bounds__(64 * kWaves<D>) void attn_decode(DecArgs a) {
 
 template <int KIND, int D, int RT>
 constexpr int lds_bytes() {
-  constexpr int q = Num<KIND>::NS * RT * (D / 32) * 1024, j = kWaves<D> * 16 * RT * (D + 4) * 4;
+  constexpr int q = Num<KIND>::NS * RT * (D / 32) * 1024, j = NW * 16 * RT * (D + 4) * 4;
   return q > j ? q : j;
 }
 
@@ -617,11 +622,11 @@ void each(F &&f) {  // every instance
 
 }  // namespace
 
-int decode_grid() {
+int decode_grid(int D) {
   int dev = 0, cus = 0;
   IJ_HIP(hipGetDevice(&dev));
   IJ_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-  return std::min(cus, kJoin * kJoin);  // (256 on an MI355X) joins of joins are one level
+  return std::min(cus * per_cu(D), kJoin * kJoins);  // (256 CUs on an MI355X)
 }
 
 void launch_attn_decode(const DecArgs &a, hipStream_t s) {
@@ -630,7 +635,7 @@ void launch_attn_decode(const DecArgs &a, hipStream_t s) {
   each([&](auto kind, auto dim, auto tiles) {
     if (a.kind == kind && a.D == dim && rt == tiles)
       hipLaunchKernelGGL((attn_decode<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>), dim3(a.W),
-                         dim3(64 * kWaves<decltype(dim)::value>),
+                         dim3(NT),
                          (lds_bytes<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>()), s, a);
   });
   IJ_HIP(hipGetLastError());

@@ -152,7 +152,7 @@ NE_API ne_kv *ne_kv_create(const ne_kv_desc *d) {
     auto kv = std::make_unique<ne_kv>();
     kv->d = *d;
     kv->kind = d->dtype == NE_BF16 ? kKvBf16 : d->dtype == NE_F16 ? kKvF16 : kKvI8;
-    kv->W = decode_grid();
+    kv->W = decode_grid(d->dim);
     const uint64_t per_page = (uint64_t)d->heads * kv_block_bytes(kv->kind, d->dim);  // < 2^33
     IJ_CHECK(per_page <= (1ull << 46) / (uint64_t)d->pages / (uint64_t)d->layers, "cache of %d layers, %d pages, %d heads",
              d->layers, d->pages, d->heads);

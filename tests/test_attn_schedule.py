@@ -84,7 +84,7 @@ static void pieces(std::mt19937 &r) {
 static void shares(std::mt19937 &r) {
   for (int it = 0; it < 3000; it++) {
     Batch b = batch(r, 1 + r() % 30, 1 + r() % (it % 5 ? 900 : 60000), 1 + r() % 8, it % 2);
-    const int W = 1 + r() % 256, H = 1 + r() % 8, group = 1 + r() % 20, BR = r() % 2 ? 16 : 32, least = r() % 2 ? 4 : 8;
+    const int W = 1 + r() % (kJoin * kJoins), H = 1 + r() % 8, group = 1 + r() % 20, BR = r() % 2 ? 16 : 32, least = r() % 2 ? 4 : 8;
     // the two forms, as the kernel chooses them
     auto total = [&](int pad) {
       int t = 0;
@@ -119,7 +119,7 @@ static void shares(std::mt19937 &r) {
           CHECK(p0 < p1 || (q.len == 0 && p0 == 0));
           real += std::max(p1 - p0, 0);
           const DecPart p = dec_part(g0, g1, share, w);
-          CHECK(p.first == first && p.parts == last - first + 1 && p.parts <= kJoin * kJoin);
+          CHECK(p.first == first && p.parts == last - first + 1 && p.parts <= kJoin * kJoins);
           if (p.parts > 1) {
             CHECK(p.slot >= 0 && p.slot < 2 * W && slots.insert(p.slot).second);
             CHECK(p.slot == dec_slot(p, g0, share, w - first));
