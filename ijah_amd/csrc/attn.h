@@ -84,47 +84,54 @@ IJ_HD int64_t kv_max_pieces(int n, int R, bool rows) {
 }
 
 // ------------------------------------------------------------------------------------------------ decode's work
-// The batch's work in units of one page for one key head and one block of query rows, in the order (sequence, key head, row
-// block, page); every sequence with rows has at least one unit per head and block (an empty one writes its zeros). A (sequence,
-// head, block) is a group. The W workgroups take consecutive shares, in one of two forms:
-//   - few units: each group is filled up to a multiple of `least` units (a page for every wave of a workgroup), and a share is
-//     `least` of them, so that no workgroup has more than one group's, and none more than a page per wave;
-//   - else equal shares of ceil(units / W), whatever the lengths.
+// The batch's work in units of a page for one wave: of one page, one key head and one or two blocks of query rows (two: two
+// units, the workgroup's waves split between them, so that their reads of a page meet in the caches), in the order (sequence,
+// key head, blocks, page). A (sequence, head, blocks) is a group; a sequence with rows has at least one page (an empty one
+// writes its zeros). The W workgroups take consecutive shares, in one of two forms:
+//   - aligned: each group is cut into chunks of C units, a workgroup takes one chunk;
+//   - else equal shares of ceil(units / W), whatever the lengths: a workgroup may end one group and begin others.
 // A group that lies in several shares is joined from one partial each: workgroup w's first segment is in slot 2w, one that
 // begins inside its share in 2w + 1. Parts are joined kJoin at a time by the last of them to finish, into the first one's slot
 // (whose number names the counter), and these by the last of their joins (at most one group that is continued begins in a
 // share, so its first workgroup names that counter): one workgroup reading all of a long sequence's parts would take longer
 // than its pages do.
 struct DecSeq {
-  int pages, blocks;  // pages (at least one), row blocks
+  int pages, nb, blocks;  // pages (at least one); row blocks of a group (1 or 2); groups per key head
 };
-IJ_HD DecSeq dec_seq(const KvSeq &q, int group, int block_rows) {
+IJ_HD DecSeq dec_seq(const KvSeq &q, int group, int block_rows, int most_nb) {
   DecSeq d;
+  const int rows = q.nr * group;
   d.pages = q.len > 0 ? (q.len + kKvPage - 1) / kKvPage : 1;
-  d.blocks = (q.nr * group + block_rows - 1) / block_rows;
+  d.nb = rows > block_rows ? most_nb : 1;
+  d.blocks = (rows + block_rows * d.nb - 1) / (block_rows * d.nb);
   return d;
 }
-IJ_HD int dec_units(const DecSeq &d, int H, int pad) { return (d.pages + pad - 1) / pad * pad * d.blocks * H; }
-// the most units that a batch can have, filled up: the host refuses batches where this passes 31 bits
-IJ_HD int64_t dec_max_units(int n, int ldt, int R, int group, int H, int block_rows, int pad) {
-  return ((int64_t)R * group / block_rows + n) * H * ((int64_t)ldt + pad);
+IJ_HD int dec_group(const DecSeq &d) { return d.pages * d.nb; }                    // units of a group
+IJ_HD int dec_chunks(const DecSeq &d, int C) { return (dec_group(d) + C - 1) / C; }  // its chunks
+IJ_HD int dec_units(const DecSeq &d, int H) { return dec_group(d) * d.blocks * H; }
+// a segment's pages: those whose first unit lies in it (the last share of a group may have none)
+IJ_HD int dec_page(const DecSeq &d, int unit, int real_pages) {
+  const int p = (unit + d.nb - 1) / d.nb;
+  return p < real_pages ? p : real_pages;
+}
+// the most units that a batch can have: the host refuses batches where this passes 31 bits
+IJ_HD int64_t dec_max_units(int n, int ldt, int R, int group, int H, int block_rows) {
+  return ((int64_t)R * group / block_rows + n) * H * 2 * ((int64_t)ldt + 1);
 }
 constexpr int kJoin = 16, kJoins = 32;  // parts of a join, joins of a join of joins: W <= kJoin kJoins
 struct DecPart {
-  int first, parts, slot;  // the group's first workgroup, how many it has, this one's partial slot
+  int first, parts, odd;  // the group's first workgroup, how many it has, whether the first one's slot is its second
 };
-// the group of units [g0, g1) seen from workgroup w
-IJ_HD DecPart dec_part(int g0, int g1, int share, int w) {
+IJ_HD DecPart dec_part_chunk(int chunk, int chunks, int w) { return DecPart{w - chunk, chunks, 0}; }
+// the group of units [g0, g1) in shares
+IJ_HD DecPart dec_part_share(int g0, int g1, int share) {
   DecPart p;
   p.first = g0 / share;
   p.parts = (g1 - 1) / share - p.first + 1;
-  p.slot = 2 * w + (w == p.first && g0 != p.first * share ? 1 : 0);
+  p.odd = g0 != p.first * share ? 1 : 0;
   return p;
 }
-// part k's slot
-IJ_HD int dec_slot(const DecPart &p, int g0, int share, int k) {
-  return 2 * (p.first + k) + (k == 0 && g0 != p.first * share ? 1 : 0);
-}
+IJ_HD int dec_slot(const DecPart &p, int k) { return 2 * (p.first + k) + (k == 0 ? p.odd : 0); }  // part k's slot
 
 // ------------------------------------------------------------------------------------------------ launches
 enum { kRowF32 = 0, kRowBf16 = 1, kRowF16 = 2 };  // a row matrix's type
@@ -150,7 +157,7 @@ struct DecArgs {
   uint32_t *cnt;   // [3 W], zero between launches: by slot of a join's first part, then by first workgroup of a group
   int W;
 };
-constexpr int kDecRows = 32;  // query rows of a block at most (the partial slots' size)
+constexpr int kDecRows = 64;  // query rows of a group at most (the partial slots' size)
 IJ_HD constexpr int dec_slot_floats(int D) { return kDecRows * (D + 2); }
 struct PromptArgs {
   int n, Hq, H, D, type, Rq, Rk;

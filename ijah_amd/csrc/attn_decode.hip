@@ -86,17 +86,17 @@ __device__ __forceinline__ void part_store(__amdgpu_buffer_rsrc_t r, uint32_t at
   __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, (int)at, 0, 16);
 }
 
-// the batch's place where a workgroup's share begins, and its walk from group to group
+// the place of a segment in the batch
 struct Group {
-  int b, h, rb;  // sequence, key head, block of query rows
+  int b, h, rb;  // sequence, key head, which of the sequence's row groups
   KvSeq q;
   DecSeq d;
-  int u0;        // the group's first unit
+  int u0;        // the group's first unit (shares), or 0
 };
 
 template <int KIND, int D, int RT>
 __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
-  constexpr int NS = Num<KIND>::NS, BR = 16 * RT;
+  constexpr int NS = Num<KIND>::NS, BR = 16 * RT, NB = RT;  // NB: row blocks of a group at most
   constexpr int KC = D / 32;                       // products of 32 dims
   constexpr int KG = KIND == kKvI8 ? KC / 2 : KC;  // granules of 16 keys
   constexpr int DB = D / 16;
@@ -106,14 +106,16 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
   constexpr float kLift = F16 ? 14.f : 0.f;
   constexpr bool kAhead = RT == 1;  // the next page's keys are requested a page ahead (two row tiles leave no registers)
   constexpr int kPitch = D + 4;     // of a row of sums in LDS
-  // LDS: the query parts [NS][RT][KC][64 lanes] granules, then the waves' sums [NW][BR][kPitch] for their join
+  // LDS: the query parts [NS][NB][RT][KC][64 lanes] granules; then the waves' sums [NW][BR][kPitch] for their join; then the
+  // maxima and sums of the parts that are joined
   extern __shared__ __align__(16) uint8_t lds[];
   u32x4 *qf = (u32x4 *)lds;
   float *js = (float *)lds;
   __shared__ int sum[NW + 2];
-  __shared__ float wm[NW][BR], wl[NW][BR], pm[kJoins][BR], pl[kJoins][BR];
+  __shared__ float wm[NW][BR], wl[NW][BR];
+  float(*pm)[NB * BR] = (float(*)[NB * BR])lds, (*pl)[NB * BR] = pm + kJoins;
   __shared__ int flag;
-  __shared__ uint32_t qmax[BR];
+  __shared__ uint32_t qmax[NB * BR];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4,
             col = lane & 15;
@@ -124,38 +126,103 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
                                 : load8<kRowF16>(a.q, row, c);
   };
   // ---- the share
-  int pad = NW;
-  auto units = [&](int b) { return dec_units(dec_seq(kv_seq(a.s, b), group, BR), a.H, pad); };
-  BatchScan<NT> sc = scan_batch<NT>(a.s.n, sum, units);
-  int share = NW;
-  if (sc.total > W * NW) {
-    pad = 1;
-    sc = scan_batch<NT>(a.s.n, sum, units);
-    share = (int)(((uint32_t)sc.total + (uint32_t)W - 1) / (uint32_t)W);
-  }
-  if ((int64_t)share * me >= sc.total) return;
-  const int u_lo = share * me, u_hi = share < sc.total - u_lo ? u_lo + share : sc.total;
+  auto seq_of = [&](int b) { return dec_seq(kv_seq(a.s, b), group, BR, NB); };
+  bool aligned = false;
+  int C = 0, chunk = 0, share = 0, u_hi = 0, u = 0;
   Group g;
-  int before;
-  g.b = find_item<NT>(sc, a.s.n, u_lo, sum, &before, units);
-  g.q = kv_seq(a.s, g.b);
-  g.d = dec_seq(g.q, group, BR);
-  int size = dec_units(g.d, 1, pad) / max(g.d.blocks, 1);  // the group's units
   {
-    const int k = (u_lo - before) / size;
-    g.h = k / g.d.blocks;
-    g.rb = k - g.h * g.d.blocks;
-    g.u0 = before + k * size;
+    int before, k;
+    if (a.s.n <= kWaveScan) {
+      // every wave for itself; a lane holds up to kPer consecutive sequences
+      constexpr int kPer = kWaveScan / 64;
+      const int per = (a.s.n + 63) >> 6;
+      int un[kPer], gr[kPer], all = 0, groups = 0;  // units of a group, groups; of the lane's sequences
+#pragma unroll
+      for (int i = 0; i < kPer; i++) {
+        const int b = lane * per + i;
+        un[i] = gr[i] = 0;
+        if (i < per && b < a.s.n) {
+          const DecSeq d = seq_of(b);
+          un[i] = dec_group(d);
+          gr[i] = d.blocks * a.H;
+        }
+        all += un[i] * gr[i];
+        groups += gr[i];
+      }
+      int mine = all, inc = wave_scan(mine);
+      all = __builtin_amdgcn_readlane(inc, 63);
+      groups = __builtin_amdgcn_readlane(wave_scan(groups), 63);
+      if (all == 0) return;
+      share = (int)(((uint32_t)all + (uint32_t)W - 1) / (uint32_t)W);
+      // chunks of up to four pages a wave more than an equal share, if the groups then fit the workgroups: a second segment
+      // (its first loads, its join) costs a workgroup about as much as three more pages for each wave
+      if (groups <= W) {
+        C = (share + NW - 1) / NW * NW;
+        for (int t = 0; t < 4 && !aligned; t++, C += aligned ? 0 : NW) {
+          int m = 0;
+#pragma unroll
+          for (int i = 0; i < kPer; i++) m += (int)((uint32_t)(un[i] + C - 1) / (uint32_t)C) * gr[i];
+          const int c = wave_scan(m);
+          if (__builtin_amdgcn_readlane(c, 63) <= W) {
+            aligned = true;
+            mine = m;
+            inc = c;
+            all = __builtin_amdgcn_readlane(c, 63);
+          }
+        }
+      }
+      const int item = aligned ? me : share * me;
+      if (item >= all) return;
+      if (!aligned) {
+        u = item;
+        u_hi = share < all - u ? u + share : all;
+      }
+      int at = inc - mine, b = lane * per;
+      const uint64_t holds = __ballot(item >= at && item < at + mine);
+#pragma unroll
+      for (int i = 0; i < kPer; i++) {
+        const int k = (aligned ? (int)((uint32_t)(un[i] + C - 1) / (uint32_t)C) : un[i]) * gr[i];
+        if (i + 1 < per && item >= at + k && b == lane * per + i) {
+          at += k;
+          b++;
+        }
+      }
+      const int from = (int)__builtin_ctzll(holds | 1ull << 63);
+      g.b = __builtin_amdgcn_readlane(b, from);
+      before = __builtin_amdgcn_readlane(at, from);
+      k = item - before;
+    } else {
+      auto units = [&](int b) { return dec_units(seq_of(b), a.H); };
+      const BatchScan<NT> sc = scan_batch<NT>(a.s.n, sum, units);
+      share = (int)(((uint32_t)sc.total + (uint32_t)W - 1) / (uint32_t)W);
+      if (share * (int64_t)me >= sc.total) return;
+      u = share * me;
+      u_hi = share < sc.total - u ? u + share : sc.total;
+      g.b = find_item<NT>(sc, a.s.n, u, sum, &before, units);
+      k = u - before;
+    }
+    g.q = kv_seq(a.s, g.b);
+    g.d = dec_seq(g.q, group, BR, NB);
+    const int size = aligned ? dec_chunks(g.d, C) : dec_group(g.d), i = k / size;
+    g.h = i / g.d.blocks;
+    g.rb = i - g.h * g.d.blocks;
+    g.u0 = aligned ? 0 : before + i * size;
+    chunk = k - i * size;
   }
-  int u = u_lo;
-  for (;;) {  // one segment: the units [u, end) of group g
-    const int g1 = g.u0 + size, end = min(g1, u_hi);
-    const int pg0 = u - g.u0, pg1 = min(end - g.u0, (g.q.len + kKvPage - 1) / kKvPage);  // its pages (none: an empty sequence)
-    const int nrows = min(g.q.nr * group - g.rb * BR, BR);
+  for (;;) {  // one segment
+    const int size = dec_group(g.d), lo = aligned ? chunk * C : u - g.u0,
+              hi = aligned ? min(lo + C, size) : min(u_hi - g.u0, size);  // its units of the group
+    const int real = (g.q.len + kKvPage - 1) / kKvPage;  // pages (none: an empty sequence)
+    const int pg0 = dec_page(g.d, lo, real), pg1 = dec_page(g.d, hi, real);
+    const DecPart part = aligned ? dec_part_chunk(chunk, dec_chunks(g.d, C), me) : dec_part_share(g.u0, g.u0 + size, share);
+    const int nb = g.d.nb, row0 = g.rb * nb * BR, nrows = min(g.q.nr * group - row0, nb * BR);  // the group's rows
+    // the wave's row block and its turn at the pages: every (NW / nb)-th
+    const int wb = nb == 1 ? 0 : wave & 1, ws = nb == 1 ? wave : wave >> 1, step = nb == 1 ? NW : NW / 2;
+    const int wrow0 = row0 + wb * BR, wrows = nrows - wb * BR;
     const int *table = a.s.table + (int64_t)g.b * a.s.ldt;
-    const int turns = pg0 + wave < pg1 ? (pg1 - pg0 - wave + NW - 1) / NW : 0;  // of this wave, which has every NW-th page
+    const int turns = pg0 + ws < pg1 ? (pg1 - pg0 - ws + step - 1) / step : 0;
     // the page ids of the wave's next 64 turns, one a lane
-    auto load_ids = [&](int t) { return table[min(pg0 + wave + (t + lane) * NW, pg1 - 1)]; };
+    auto load_ids = [&](int t) { return table[min(pg0 + ws + (t + lane) * step, pg1 - 1)]; };
     int ids = 0, id = 0;
     u32x4 kf[4][KG], vf[DB][VG];
     auto valid = [&](int i) { return i >= 0 && i < a.s.pages; };
@@ -172,15 +239,16 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
       id = __builtin_amdgcn_readlane(ids, 0);
       if constexpr (kAhead) load_keys(id);
     }
-    // ---- the block's query rows, scaled, in parts: granule (part, tile, chunk, lane) = 8 dims of row `col`
-    constexpr int QN = (RT * KC * 64 + NT - 1) / NT;
+    // ---- the group's query rows, scaled, in parts: granule (part, block, tile, chunk, lane) = 8 dims of row `col`
+    constexpr int kTile = KC * 64, QN = (NB * RT * kTile + NT - 1) / NT, kPart = NB * RT * kTile;
+    const int granules = nb * RT * kTile;
     f32x8 x[QN];
 #pragma unroll
     for (int n = 0; n < QN; n++) {
-      const int i = n * NT + tid, m = (i / (KC * 64)) * 16 + (i & 15), c = (i >> 6) % KC, qd = (i >> 4) & 3;
+      const int i = n * NT + tid, m = i / kTile * 16 + (i & 15), c = (i >> 6) % KC, qd = (i >> 4) & 3;
       const int d = KIND == kKvI8 ? (c >> 1) * 64 + qd * 16 + (c & 1) * 8 : c * 32 + qd * 8;
-      if (i < RT * KC * 64 && m < nrows) {
-        const int row = g.rb * BR + m, t = row / group;
+      if (i < granules && m < nrows) {
+        const int row = row0 + m, t = row / group;
         x[n] = load_q(g.q.r0 + t, (g.h * group + row - t * group) * D + d);
       } else {
 #pragma unroll
@@ -189,7 +257,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
     }
     __syncthreads();  // the segment before has left LDS
     if constexpr (F16) {
-      if (tid < BR) qmax[tid] = 0;
+      if (tid < NB * BR) qmax[tid] = 0;
       __syncthreads();
 #pragma unroll
       for (int n = 0; n < QN; n++) {
@@ -197,7 +265,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         uint32_t top = 0;
 #pragma unroll
         for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(x[n][k]) & 0x7FFFFFFFu);
-        if (i < RT * KC * 64) atomicMax(&qmax[(i / (KC * 64)) * 16 + (i & 15)], top);
+        if (i < granules) atomicMax(&qmax[i / kTile * 16 + (i & 15)], top);
       }
       __syncthreads();
     }
@@ -208,25 +276,27 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
 #pragma unroll
     for (int n = 0; n < QN; n++) {
       const int i = n * NT + tid;
-      if (i >= RT * KC * 64) break;
-      if constexpr (F16) {
-        const int e = -q_exp((i / (KC * 64)) * 16 + (i & 15));
+      if (i < granules) {
+        if constexpr (F16) {
+          const int e = -q_exp(i / kTile * 16 + (i & 15));
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[n][k] = __builtin_amdgcn_ldexpf(x[n][k], e);
+          for (int k = 0; k < 8; k++) x[n][k] = __builtin_amdgcn_ldexpf(x[n][k], e);
+        }
+#pragma unroll
+        for (int p = 0; p < NS; p++) qf[p * kPart + i] = part_of<KIND>(x[n]);
       }
-#pragma unroll
-      for (int p = 0; p < NS; p++) qf[p * RT * KC * 64 + i] = part_of<KIND>(x[n]);
     }
+    const u32x4 *wq = qf + wb * RT * kTile + lane;  // the wave's
     // the last token that row col of tile t sees
     int seen[RT];
     float scale[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-      scale[t] = F16 ? __builtin_amdgcn_ldexpf(a.scale, q_exp(t * 16 + col)) : a.scale;
-      const int row = g.rb * BR + t * 16 + col;
-      seen[t] = t * 16 + col < nrows ? g.q.len - g.q.nr + row / group : -1;
+      scale[t] = F16 ? __builtin_amdgcn_ldexpf(a.scale, q_exp(wb * BR + t * 16 + col)) : a.scale;
+      const int row = wrow0 + t * 16 + col;
+      seen[t] = t * 16 + col < wrows ? g.q.len - g.q.nr + row / group : -1;
     }
-    const int all_see = g.q.len - g.q.nr + g.rb * BR / group;  // every row of the block sees up to here
+    const int all_see = g.q.len - g.q.nr + wrow0 / group;  // every row of the block sees up to here
     f32x4 o[RT][DB];
     float mx[RT], l[RT];
     int ve = -200;  // 8 bits: the power of two that the sums are in units of (below any step's)
@@ -239,7 +309,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
     }
     __syncthreads();
     for (int it = 0; it < turns; it++) {
-      const int pg = pg0 + wave + it * NW;
+      const int pg = pg0 + ws + it * step;
       const uint8_t *blk = block(id);
       const u32x4 *vp = (const u32x4 *)(blk + kKvPage * D * kv_esize(KIND)) + lane;
       const bool there = valid(id);  // a page id outside the pool: a page that nobody sees
@@ -273,12 +343,12 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         for (int kb = 0; kb < 4; kb++) s[t][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < KC; c++) {
-        if constexpr (KIND == kKvI8 && RT > 1) __builtin_amdgcn_sched_barrier(0);  // (no conversions ahead: registers)
+        if constexpr (RT > 1 && (KIND == kKvI8 || D == 256)) __builtin_amdgcn_sched_barrier(0);  // (nothing ahead: registers)
 #pragma unroll
         for (int t = 0; t < RT; t++)
 #pragma unroll
           for (int p = NS - 1; p >= 0; p--) {
-            const u32x4 b = qf[((p * RT + t) * KC + c) * 64 + lane];
+            const u32x4 b = wq[p * kPart + (t * KC + c) * 64];
 #pragma unroll
             for (int kb = 0; kb < 4; kb++) {
               u32x4 k;
@@ -452,7 +522,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
           for (int k = 0; k < 4; k++) o[t][i][k] = __builtin_amdgcn_ldexpf(o[t][i][k], ve);
     }
     // ---- the segment's waves joined
-    const int used = max(min(NW, pg1 - pg0), 1);  // waves that had a page; one has the zeros of an empty sequence
+    const int used = max(min(step, pg1 - pg0), 1);  // waves of a block that had a page; one has the zeros of none
     __syncthreads();  // every wave has read its query parts
 #pragma unroll
     for (int t = 0; t < RT; t++) {
@@ -463,16 +533,17 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         wm[wave][t * 16 + col] = mx[t];
         wl[wave][t * 16 + col] = s;
       }
-      if (wave < used && t * 16 + col < nrows) {
+      if (ws < used && t * 16 + col < wrows) {
 #pragma unroll
         for (int i = 0; i < DB; i++) *(f32x4 *)(js + (wave * BR + t * 16 + col) * kPitch + i * 16 + quad * 4) = o[t][i];
       }
     }
     __syncthreads();
-    const DecPart part = dec_part(g.u0, g1, share, me);
+    const int slot = dec_slot(part, me - part.first) * SLOT;  // in floats
+    constexpr int ROWS = NB * BR;
     const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)(2u * W * SLOT * 4), 0x00020000);
     auto out4 = [&](int m, int d, f32x4 v) {  // four output elements
-      const int row = g.rb * BR + m, t = row / group;
+      const int row = row0 + m, t = row / group;
       const int64_t at = (g.q.r0 + t) * a.out.ld + (g.h * group + row - t * group) * D + d;
       if (a.type == kRowF32) {
         *(f32x4 *)((float *)a.out.p + at) = v;
@@ -494,20 +565,21 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
     };
     for (int i = tid; i < nrows * (D / 4); i += NT) {
       const int m = i / (D / 4), d = i % (D / 4) * 4;
+      const int w0 = m / BR, mm = m - w0 * BR;  // the waves w0, w0 + nb, .. hold the row
       float top = kNegInf, s = 0.f;
-      for (int w = 0; w < used; w++) top = fmaxf(top, wm[w][m]);
+      for (int w = 0; w < used; w++) top = fmaxf(top, wm[w0 + w * nb][mm]);
       const float ms = top == kNegInf ? 0.f : top;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
       for (int w = 0; w < used; w++) {
-        const float f = __builtin_amdgcn_exp2f(wm[w][m] - ms);
-        s = __builtin_fmaf(wl[w][m], f, s);
-        v += *(const f32x4 *)(js + (w * BR + m) * kPitch + d) * f;
+        const float f = __builtin_amdgcn_exp2f(wm[w0 + w * nb][mm] - ms);
+        s = __builtin_fmaf(wl[w0 + w * nb][mm], f, s);
+        v += *(const f32x4 *)(js + ((w0 + w * nb) * BR + mm) * kPitch + d) * f;
       }
       if (part.parts > 1) {
-        part_store(parts, (uint32_t)(part.slot * SLOT + m * D + d) * 4u, v);
+        part_store(parts, (uint32_t)(slot + m * D + d) * 4u, v);
         if (d == 0) {
-          st_cg(a.part + (int64_t)part.slot * SLOT + BR * D + m, top);
-          st_cg(a.part + (int64_t)part.slot * SLOT + BR * D + BR + m, s);
+          st_cg(a.part + slot + ROWS * D + m, top);
+          st_cg(a.part + slot + ROWS * D + ROWS + m, s);
         }
       } else {
         out4(m, d, v * (s == 0.f ? 0.f : 1.f / s));
@@ -515,14 +587,14 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
     }
     // ---- the group's shares joined: parts by kJoin, then their joins
     if (part.parts > 1) {
-      // parts k0, k0 + step, .. (cnt of them) into part k0's slot, or into the output
-      auto join = [&](int k0, int step, int cnt, bool final) {
-        for (int i = tid; i < cnt * BR; i += NT) {
-          const int k = i / BR, m = i % BR;
+      // parts k0, k0 + every, .. (cnt of them) into part k0's slot, or into the output
+      auto join = [&](int k0, int every, int cnt, bool final) {
+        for (int i = tid; i < cnt * ROWS; i += NT) {
+          const int k = i / ROWS, m = i % ROWS;
           if (m < nrows) {
-            const float *sl = a.part + (int64_t)dec_slot(part, g.u0, share, k0 + k * step) * SLOT + BR * D;
+            const float *sl = a.part + dec_slot(part, k0 + k * every) * SLOT + ROWS * D;
             pm[k][m] = ld_cg(sl + m);
-            pl[k][m] = ld_cg(sl + BR + m);
+            pl[k][m] = ld_cg(sl + ROWS + m);
           }
         }
         __syncthreads();
@@ -533,8 +605,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
           for (int r = 0; r < cnt; r += kJoin) {
 #pragma unroll
             for (int k = 0; k < kJoin; k++)  // all requested at once; behind the last the first again, not used
-              in[k] = part_load(parts, (uint32_t)(dec_slot(part, g.u0, share, k0 + (r + k < cnt ? r + k : 0) * step) * SLOT +
-                                                  m * D + d) * 4u);
+              in[k] = part_load(parts, (uint32_t)(dec_slot(part, k0 + (r + k < cnt ? r + k : 0) * every) * SLOT + m * D + d) * 4u);
             if (r == 0)
               for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][m]);
             const float ms = top == kNegInf ? 0.f : top;
@@ -550,11 +621,11 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
           if (final) {
             out4(m, d, v * (s == 0.f ? 0.f : 1.f / s));
           } else {
-            const int to = dec_slot(part, g.u0, share, k0) * SLOT;
+            const int to = dec_slot(part, k0) * SLOT;
             part_store(parts, (uint32_t)(to + m * D + d) * 4u, v);
             if (d == 0) {
-              st_cg(a.part + to + BR * D + m, top);
-              st_cg(a.part + to + BR * D + BR + m, s);
+              st_cg(a.part + to + ROWS * D + m, top);
+              st_cg(a.part + to + ROWS * D + ROWS + m, s);
             }
           }
         }
@@ -571,7 +642,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
       };
       const int k = me - part.first, k0 = k / kJoin * kJoin, cnt = min(part.parts - k0, kJoin);
       const bool one = part.parts <= kJoin;
-      if (cnt == 1 || last_of(a.cnt + dec_slot(part, g.u0, share, k0), cnt)) {
+      if (cnt == 1 || last_of(a.cnt + dec_slot(part, k0), cnt)) {
         if (cnt > 1) join(k0, 1, cnt, one);
         if (!one) {
           const int joins = (part.parts + kJoin - 1) / kJoin;  // at most kJoins
@@ -579,10 +650,10 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         }
       }
     }
-    if (end == u_hi) return;
+    if (aligned || g.u0 + hi == u_hi) return;
     // ---- the next group
-    u = end;
-    g.u0 = end;
+    g.u0 += size;
+    u = g.u0;
     if (++g.rb == g.d.blocks) {
       g.rb = 0;
       if (++g.h == a.H) {
@@ -590,9 +661,8 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         do {
           if (++g.b >= a.s.n) return;  // (not reached: u < total, so a later sequence has rows)
           g.q = kv_seq(a.s, g.b);
-          g.d = dec_seq(g.q, group, BR);
+          g.d = dec_seq(g.q, group, BR, NB);
         } while (!g.d.blocks);
-        size = dec_units(g.d, 1, pad) / g.d.blocks;
       }
     }
   }
@@ -600,8 +670,8 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
 
 template <int KIND, int D, int RT>
 constexpr int lds_bytes() {
-  constexpr int q = Num<KIND>::NS * RT * (D / 32) * 1024, j = NW * 16 * RT * (D + 4) * 4;
-  return q > j ? q : j;
+  constexpr int q = Num<KIND>::NS * RT * RT * (D / 32) * 1024, j = NW * 16 * RT * (D + 4) * 4, p = 2 * kJoins * 16 * RT * RT * 4;
+  return q > j ? (q > p ? q : p) : (j > p ? j : p);
 }
 
 template <typename F>

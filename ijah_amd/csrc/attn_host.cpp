@@ -201,7 +201,7 @@ NE_API int ne_attn_decode(ne_kv *kv, int layer, const ne_kv_seqs *s, int R, int 
     check_scale(scale);
     DecArgs a;
     a.s = seqs_of(kv, s, R);
-    IJ_CHECK(dec_max_units(s->n, s->ldt, R, heads / kv->d.heads, kv->d.heads, 16, 8) < (1ll << 31) &&
+    IJ_CHECK(dec_max_units(s->n, s->ldt, R, heads / kv->d.heads, kv->d.heads, 16) < (1ll << 31) &&
                  (int64_t)R * heads < (1ll << 31),
              "%d rows of %d heads over %d tables of %d pages: too much for one call", R, heads, s->n, s->ldt);
     a.kind = kv->kind;

@@ -84,54 +84,62 @@ static void pieces(std::mt19937 &r) {
 static void shares(std::mt19937 &r) {
   for (int it = 0; it < 3000; it++) {
     Batch b = batch(r, 1 + r() % 30, 1 + r() % (it % 5 ? 900 : 60000), 1 + r() % 8, it % 2);
-    const int W = 1 + r() % (kJoin * kJoins), H = 1 + r() % 8, group = 1 + r() % 20, BR = r() % 2 ? 16 : 32, least = r() % 2 ? 4 : 8;
-    // the two forms, as the kernel chooses them
-    auto total = [&](int pad) {
-      int t = 0;
-      for (int i = 0; i < b.s.n; i++) t += dec_units(dec_seq(kv_seq(b.s, i), group, BR), H, pad);
-      CHECK(t <= dec_max_units(b.s.n, b.s.ldt, b.s.R, group, H, 16, 8));
-      return t;
-    };
-    int pad = least, all = total(pad), share = least;
-    if (all > W * least) {
-      pad = 1;
-      all = total(pad);
-      share = (all + W - 1) / W;
-    }
-    if (!all) continue;
-    CHECK((int64_t)share * W >= all);
-    std::set<int> slots, counters, firsts;
-    int64_t units = 0;
-    int at = 0;
+    const int W = 1 + r() % (kJoin * kJoins), H = 1 + r() % 8, group = 1 + r() % 20, NB = 1 + r() % 2, BR = 16 * NB;
+    int64_t all = 0, groups = 0;
     for (int i = 0; i < b.s.n; i++) {
-      const KvSeq q = kv_seq(b.s, i);
-      const DecSeq d = dec_seq(q, group, BR);
-      CHECK(d.pages >= 1 && d.blocks >= 0);
-      for (int k = 0; k < H * d.blocks; k++) {
-        const int g0 = at, g1 = g0 + dec_units(d, 1, pad) / d.blocks, first = g0 / share, last = (g1 - 1) / share;
-        at = g1;
-        CHECK(last < W);
-        int real = 0;
-        for (int w = first; w <= last; w++) {
-          const int lo = std::max(g0, share * w), hi = std::min(g1, share * (w + 1));
-          CHECK(lo < hi);
-          const int p0 = lo - g0, p1 = std::min(hi - g0, (q.len + kKvPage - 1) / kKvPage);
-          CHECK(p0 < p1 || (q.len == 0 && p0 == 0));
-          real += std::max(p1 - p0, 0);
-          const DecPart p = dec_part(g0, g1, share, w);
-          CHECK(p.first == first && p.parts == last - first + 1 && p.parts <= kJoin * kJoins);
-          if (p.parts > 1) {
-            CHECK(p.slot >= 0 && p.slot < 2 * W && slots.insert(p.slot).second);
-            CHECK(p.slot == dec_slot(p, g0, share, w - first));
-            if ((w - first) % kJoin == 0) CHECK(counters.insert(p.slot).second);
-          }
-        }
-        CHECK(real == (q.len + kKvPage - 1) / kKvPage);
-        units += g1 - g0;
-        if (last > first) CHECK(firsts.insert(first).second);
-      }
+      const DecSeq d = dec_seq(kv_seq(b.s, i), group, BR, NB);
+      CHECK(d.pages >= 1 && d.blocks >= 0 && d.nb >= 1 && d.nb <= NB);
+      CHECK((int64_t)d.blocks * d.nb * BR >= (int64_t)kv_seq(b.s, i).nr * group);
+      all += dec_units(d, H);
+      groups += d.blocks * H;
     }
-    CHECK(units == all && at == all);
+    CHECK(all <= dec_max_units(b.s.n, b.s.ldt, b.s.R, group, H, 16));
+    if (!all) continue;
+    const int share = (all + W - 1) / W;
+    for (int form = 0; form < 5; form++) {  // shares; chunks of a share and up to three times four units more
+      const int C = form ? (share + 3) / 4 * 4 + 4 * (form - 1) : 0;
+      int64_t chunks = 0;
+      if (form) {
+        for (int i = 0; i < b.s.n; i++) {
+          const DecSeq d = dec_seq(kv_seq(b.s, i), group, BR, NB);
+          chunks += (int64_t)dec_chunks(d, C) * d.blocks * H;
+        }
+        if (chunks > W) continue;
+      }
+      std::set<int> slots, counters, firsts;
+      int at = 0, item = 0;
+      for (int i = 0; i < b.s.n; i++) {
+        const KvSeq q = kv_seq(b.s, i);
+        const DecSeq d = dec_seq(q, group, BR, NB);
+        const int real = (q.len + kKvPage - 1) / kKvPage, size = dec_group(d);
+        for (int k = 0; k < H * d.blocks; k++) {
+          const int g0 = at, g1 = at + size;
+          at = g1;
+          const int first = form ? item : g0 / share, parts = form ? dec_chunks(d, C) : (g1 - 1) / share - first + 1;
+          CHECK(first + parts <= W && parts <= kJoin * kJoins);
+          int page = 0;
+          for (int p = 0; p < parts; p++) {
+            const int w = first + p;
+            const DecPart part = form ? dec_part_chunk(p, parts, w) : dec_part_share(g0, g1, share);
+            CHECK(part.first == first && part.parts == parts);
+            const int lo = form ? p * C : std::max(g0, share * w) - g0;
+            const int hi = form ? std::min(lo + C, size) : std::min(g1, share * (w + 1)) - g0;
+            CHECK(lo < hi);
+            CHECK(dec_page(d, lo, real) == page);  // the parts' pages follow one another
+            page = dec_page(d, hi, real);
+            if (parts > 1) {
+              const int slot = dec_slot(part, p);
+              CHECK(slot >= 0 && slot < 2 * W && slots.insert(slot).second && slot / 2 == w);
+              if (p % kJoin == 0) CHECK(counters.insert(slot).second);
+            }
+          }
+          CHECK(page == real);
+          if (parts > 1) CHECK(firsts.insert(first).second);
+          item += parts;
+        }
+      }
+      CHECK(at == all && (!form || item == chunks));
+    }
   }
 }
 int main() {
