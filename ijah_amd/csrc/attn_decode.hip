@@ -157,7 +157,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
       // chunks of up to four pages a wave more than an equal share, if the groups then fit the workgroups: a second segment
       // (its first loads, its join) costs a workgroup about as much as three more pages for each wave
       if (groups <= W) {
-        C = (share + NW - 1) / NW * NW;
+        C = max((share + NW - 1) / NW, RT == 1 ? 1 : 4) * NW;  // (many rows: a join costs more than the pages of a turn)
         for (int t = 0; t < 4 && !aligned; t++, C += aligned ? 0 : NW) {
           int m = 0;
 #pragma unroll
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         for (int kb = 0; kb < 4; kb++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            float v = s[t][kb][i] * scale[t];
+            float v = s[t][kb][i];
             if constexpr (KIND == kKvI8) v *= ks[kb][i];
             if (edge) v = j0 + kb * 16 + i <= last ? v : kNegInf;
             s[t][kb][i] = v;
@@ -414,15 +414,22 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
           }
         top = fmaxf(top, xor_lane<16>(top, lane));
         top = fmaxf(top, xor_lane<32>(top, lane));
-        const float m1 = fmaxf(mx[t], top), ms = m1 == kNegInf ? 0.f : m1, ml = ms - kLift;
-        const float alpha = __builtin_amdgcn_exp2f(mx[t] - ms);
+        // (mx: the running maximum of the products; the scale is positive and comes in with the exponentials)
+        const float m1 = fmaxf(mx[t], top), ml = (m1 == kNegInf ? 0.f : m1 * scale[t]) - kLift;
+        // (most pages change no maximum; always where the branch costs registers that are not there)
+        if (KIND == kKvI8 || (D == 256 && RT == 2) || __ballot(m1 != mx[t])) {
+          const float alpha = m1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f((mx[t] - m1) * scale[t]);
+          l[t] *= alpha;
+#pragma unroll
+          for (int i = 0; i < DB; i++) o[t][i] *= alpha * vshift;
+        }
         mx[t] = m1;
         float add = 0.f;
 #pragma unroll
         for (int kb = 0; kb < 4; kb++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            float e = __builtin_amdgcn_exp2f(s[t][kb][i] - ml);
+            float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][kb][i], scale[t], -ml));
             add += e;
             if constexpr (KIND == kKvI8) {
               e *= vs[kb][i];
@@ -430,9 +437,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
             }
             p[t][kb >> 1][(kb & 1) * 4 + i] = e;
           }
-        l[t] = l[t] * alpha + add;
-#pragma unroll
-        for (int i = 0; i < DB; i++) o[t][i] *= alpha * vshift;
+        l[t] += add;
       }
       // 16 bits: what lies behind the last token may be anything, and 0 times it too, so it is cleared. Among drafts a value
       // that is not finite must not reach the rows of earlier drafts either: it is taken out of the product, and the sums of
@@ -530,7 +535,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
       s += xor_lane<16>(s, lane);
       s += xor_lane<32>(s, lane);
       if (quad == 0) {
-        wm[wave][t * 16 + col] = mx[t];
+        wm[wave][t * 16 + col] = mx[t] * scale[t];
         wl[wave][t * 16 + col] = s;
       }
       if (ws < used && t * 16 + col < wrows) {
@@ -598,36 +603,50 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
           }
         }
         __syncthreads();
-        for (int i = tid; i < nrows * (D / 4); i += NT) {
+        if (tid < nrows) {  // each part's factor in place of its maximum, the row's maximum and sum
+          float top = kNegInf, sum = 0.f;
+          for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][tid]);
+          const float ms = top == kNegInf ? 0.f : top;
+          for (int k = 0; k < cnt; k++) {
+            const float f = __builtin_amdgcn_exp2f(pm[k][tid] - ms);
+            pm[k][tid] = f;
+            sum = __builtin_fmaf(pl[k][tid], f, sum);
+          }
+          if (!final) {
+            st_cg(a.part + dec_slot(part, k0) * SLOT + ROWS * D + tid, top);
+            st_cg(a.part + dec_slot(part, k0) * SLOT + ROWS * D + ROWS + tid, sum);
+          }
+          pl[0][tid] = sum == 0.f ? 0.f : 1.f / sum;
+        }
+        __syncthreads();
+        // four dims of a row at a time, kJoin parts' requests in flight and the next ones behind them
+        const int items = nrows * (D / 4);
+        auto request = [&](f32x4 *in, int i, int r) {
           const int m = i / (D / 4), d = i % (D / 4) * 4;
-          f32x4 v = {0.f, 0.f, 0.f, 0.f}, in[kJoin];
-          float top = kNegInf, s = 0.f;
-          for (int r = 0; r < cnt; r += kJoin) {
 #pragma unroll
-            for (int k = 0; k < kJoin; k++)  // all requested at once; behind the last the first again, not used
-              in[k] = part_load(parts, (uint32_t)(dec_slot(part, k0 + (r + k < cnt ? r + k : 0) * every) * SLOT + m * D + d) * 4u);
-            if (r == 0)
-              for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][m]);
-            const float ms = top == kNegInf ? 0.f : top;
+          for (int k = 0; k < kJoin; k++)
+            if (r + k < cnt) in[k] = part_load(parts, (uint32_t)(dec_slot(part, k0 + (r + k) * every) * SLOT + m * D + d) * 4u);
+        };
+        f32x4 in[kJoin] = {}, next[kJoin] = {}, v = {0.f, 0.f, 0.f, 0.f};
+        int i = tid, r = 0;
+        if (i < items) request(in, i, 0);
+        while (i < items) {
+          const bool done = r + kJoin >= cnt;  // the item's last round
+          const int i1 = done ? i + NT : i, r1 = done ? 0 : r + kJoin;
+          if (i1 < items) request(next, i1, r1);
+          const int m = i / (D / 4), d = i % (D / 4) * 4;
 #pragma unroll
-            for (int k = 0; k < kJoin; k++) {
-              if (r + k < cnt) {
-                const float f = __builtin_amdgcn_exp2f(pm[r + k][m] - ms);
-                s = __builtin_fmaf(pl[r + k][m], f, s);
-                v += in[k] * f;
-              }
-            }
+          for (int k = 0; k < kJoin; k++)
+            if (r + k < cnt) v += in[k] * pm[r + k][m];
+          if (done) {
+            if (final) out4(m, d, v * pl[0][m]);
+            else part_store(parts, (uint32_t)(dec_slot(part, k0) * SLOT + m * D + d) * 4u, v);
+            v = f32x4{0.f, 0.f, 0.f, 0.f};
           }
-          if (final) {
-            out4(m, d, v * (s == 0.f ? 0.f : 1.f / s));
-          } else {
-            const int to = dec_slot(part, k0) * SLOT;
-            part_store(parts, (uint32_t)(to + m * D + d) * 4u, v);
-            if (d == 0) {
-              st_cg(a.part + to + ROWS * D + m, top);
-              st_cg(a.part + to + ROWS * D + ROWS + m, s);
-            }
-          }
+#pragma unroll
+          for (int k = 0; k < kJoin; k++) in[k] = next[k];
+          i = i1;
+          r = r1;
         }
       };
       auto last_of = [&](uint32_t *c, int n) {  // every wave's stores have arrived; true in the n-th workgroup to come here
