@@ -56,10 +56,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {  // all ones in the
   constexpr uint32_t e = KIND == kKvBf16 ? 0x7F80u : 0x7C00u;
   return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
 }
-__device__ __forceinline__ int again(int v) {  // v as a value of its own from here on: computed here, not held
-  asm volatile("" : "+v"(v));
-  return v;
-}
 // x = part + rest exactly (the subtraction of a value's own rounding is exact)
 template <int KIND>
 __device__ __forceinline__ u32x4 part_of(f32x8 &x) {

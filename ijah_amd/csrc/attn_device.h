@@ -15,6 +15,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+__device__ __forceinline__ int again(int v) {  // v as a value of its own from here on: what follows is computed here, not held
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // ---- rows: 8 elements from element index i of a row matrix (16-byte aligned) as f32, and back (nearest even)
 // (the type is a template argument: with a run-time one, the compiler dropped the fp16 branch of a copy whose two conversions
 // cancel)

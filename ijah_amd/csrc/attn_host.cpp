@@ -255,6 +255,8 @@ NE_API int ne_attn_prompt(const ne_attn_prompt_desc *d, double *gpu_ms) {
     IJ_CHECK(!overlap(a.q, a.Rq, qc, a.out, a.Rq, qc, e) && !overlap(a.k, a.Rk, kc, a.out, a.Rq, qc, e) &&
                  !overlap(a.v, a.Rk, kc, a.out, a.Rq, qc, e),
              "out overlaps q, k or v");
+    IJ_CHECK(a.k.ld < (1 << 22) && a.v.ld < (1 << 22), "row strides %lld and %lld of k and v (below 2^22)",
+             (long long)a.k.ld, (long long)a.v.ld);  // (a tile's rows are addressed in 31 bits)
     a.q_rows = ints_of(d->q_rows, (uint64_t)a.n + 1, "q_rows");
     a.k_rows = d->k_rows ? ints_of(d->k_rows, (uint64_t)a.n + 1, "k_rows") : a.q_rows;
     a.scale = d->scale * kLog2e;

@@ -23,6 +23,7 @@ namespace {
 constexpr float kNegInf = -__builtin_inff();
 constexpr int kBM = 128;  // query rows of a workgroup
 
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <bool F16>
@@ -55,6 +56,45 @@ __device__ __forceinline__ int value_chunk(int j, int c) {
   return j * (D / 8) + (c ^ (D == 64 ? (((j >> 1) & 1) << 1 | ((j >> 2) & 1)) << 1 : ((j & 3) << 1 | ((j >> 2) & 1)) << 1));
 }
 
+// the 128 query rows of a workgroup: sequence, head, first row; keys: those that some row of the block sees
+struct Block {
+  int h, hk, nq, nk, i0, off, keys;
+  int64_t q0, k0;
+};
+// The last blocks of a sequence see the most keys: they go first. Workgroups go to the XCDs in turn: where the heads divide
+// by their number, an XCD takes an eighth of them, so that the heads of a group read its keys from one L2.
+__device__ __forceinline__ bool find_block(const PromptArgs &a, int *sum, Block *w) {
+  constexpr int kXcds = 8;
+  const int blocks = gridDim.x / a.Hq, id = blockIdx.x;
+  int item;
+  if (a.Hq % kXcds == 0) {
+    const int per = a.Hq / kXcds, i = id / kXcds;
+    w->h = id % kXcds * per + i % per;
+    item = blocks - 1 - i / per;
+  } else {
+    w->h = id % a.Hq;
+    item = blocks - 1 - id / a.Hq;
+  }
+  auto bound = [](const int *p, int b, int R) { return kv_clamp(p[b], 0, R); };
+  auto q_of = [&](int b) { return max(bound(a.q_rows, b + 1, a.Rq) - bound(a.q_rows, b, a.Rq), 0); };
+  auto items = [&](int i) { return (q_of(i) + kBM - 1) / kBM; };
+  const BatchScan<256> sc = scan_batch<256>(a.n, sum, items);
+  if (item >= sc.total) return false;
+  int before;
+  const int b = find_item<256>(sc, a.n, item, sum, &before, items);
+  w->nq = q_of(b);
+  w->q0 = bound(a.q_rows, b, a.Rq);
+  w->i0 = (item - before) * kBM;
+  const int k0 = bound(a.k_rows, b, a.Rk);
+  w->k0 = k0;
+  w->nk = max(bound(a.k_rows, b + 1, a.Rk) - k0, 0);
+  w->off = w->nk - w->nq;
+  w->hk = w->h / (a.Hq / a.H);
+  w->keys = min(w->nk, min(w->i0 + kBM, w->nq) + w->off);
+  return true;
+}
+
+// ------------------------------------------------------------------------------------------------ 32-bit rows
 template <int D, int BN, int NT, bool F16>
 __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
   constexpr int KC = D / 16, DB = D / 32, KB = BN / 32, CH = D / 8, kPlane = BN * D * 2;
@@ -63,22 +103,13 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
   __shared__ uint32_t odd[BN];  // keys of the tile whose value is not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5,
             col = lane & 31;
-  auto bound = [](const int *p, int b, int R) { return kv_clamp(p[b], 0, R); };
-  auto q_of = [&](int b) { return max(bound(a.q_rows, b + 1, a.Rq) - bound(a.q_rows, b, a.Rq), 0); };
-  // the last blocks see the most keys: they go first
-  const int blocks = gridDim.x / a.Hq, h = blockIdx.x % a.Hq, item = blocks - 1 - (int)blockIdx.x / a.Hq;
-  auto items = [&](int i) { return (q_of(i) + kBM - 1) / kBM; };
-  const BatchScan<256> sc = scan_batch<256>(a.n, sum, items);
-  if (item >= sc.total) return;
-  int before;
-  const int b = find_item<256>(sc, a.n, item, sum, &before, items);
-  const int nq = q_of(b), q0 = bound(a.q_rows, b, a.Rq), i0 = (item - before) * kBM;
-  const int k0 = bound(a.k_rows, b, a.Rk), nk = max(bound(a.k_rows, b + 1, a.Rk) - k0, 0);
-  const int off = nk - nq, hk = h / (a.Hq / a.H);
+  Block w;
+  if (!find_block(a, sum, &w)) return;
+  const int nq = w.nq, nk = w.nk, i0 = w.i0, off = w.off, hk = w.hk, h = w.h, keys = w.keys;
+  const int64_t q0 = w.q0, k0 = w.k0;
   const int row = i0 + wave * 32 + col;  // this lane's query row in its sequence
   const int last = row + off;            // the last key it sees
-  const int keys = min(nk, min(i0 + kBM, nq) + off);  // of the block
-  const int all_see = i0 + off;                       // every row sees up to here
+  const int all_see = i0 + off;          // every row sees up to here
 
   // the wave's query rows as B operands; three parts of 256 dims are cut again for each tile (192 registers otherwise)
   constexpr bool kCut = NT == 3 && D == 256;
@@ -111,7 +142,7 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
     // sees, a value that is not finite is cleared (0 times it is not 0) and remembered.
     if (edge && tid < BN) odd[tid] = 0;
     if (edge) __syncthreads();
-#pragma unroll(NT == 3 ? 2 : BN * CH / 256)
+#pragma unroll 2
     for (int n = 0; n < BN * CH / 256; n++) {
       const int i = n * 256 + tid, j = i / CH, c = i % CH;
       const int64_t r = k0 + min(t0 + j, nk - 1);
@@ -277,7 +308,6 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
           for (int x = 0; x < 4; x++) w[x] = (_Float16)v[x];
           *(f16x4 *)((_Float16 *)a.out.p + at) = w;
         } else {
-          typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
           bf16x4 w;
 #pragma unroll
           for (int x = 0; x < 4; x++) w[x] = (__bf16)v[x];
@@ -287,9 +317,227 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
   }
 }
 
-// keys of a tile: what three planes of 256 dims leave room for in LDS
+// ------------------------------------------------------------------------------------------------ 16-bit rows
+// Tiles go from HBM to LDS by DMA, the next one while this one is computed (two buffers, one barrier a tile). A DMA of a
+// wave fills 1 KB of LDS in lane order, so the rotation of a row's chunks is in the addresses that the lanes read from. The
+// buffer resource ends with the sequence's last key: rows behind it arrive as zeros.
+template <int D, int BN>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const RowMat &m, const Block &w, int t0) {
+  const uint64_t base = (uint64_t)((const uint16_t *)m.p + (w.k0 + t0) * m.ld + w.hk * D);
+  const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)) << 32;
+  const int bytes = __builtin_amdgcn_readfirstlane((min(w.nk - t0, BN) - 1) * (int)m.ld * 2 + D * 2);
+  return __builtin_amdgcn_make_buffer_rsrc((void *)u, (short)0, bytes, 0x00020000);
+}
+
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t at, void *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)to, 16, at, 0, 0, 0);
+}
+
+template <int D, int BN, bool F16>
+__global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
+  constexpr int KC = D / 16, DB = D / 32, KB = BN / 32, CH = D / 8, kTile = BN * D * 2, kRow = D * 2;
+  constexpr int kDma = kTile / 1024 / 4;  // of keys, and of values, by each wave
+  extern __shared__ __align__(16) uint8_t lds[];  // two buffers of keys [BN][D], values [BN][D]
+  __shared__ int sum[6];
+  __shared__ uint32_t odd[BN];  // keys of the tile whose value is not finite
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5,
+            col = lane & 31;
+  Block w;
+  if (!find_block(a, sum, &w)) return;
+  const int row = w.i0 + wave * 32 + col;  // this lane's query row in its sequence
+  const int last = row + w.off;            // the last key it sees
+  const int all_see = w.i0 + w.off;        // every row of the block sees up to here
+  const float scale = a.scale;
+
+  // ---- where this lane's DMAs read: row and chunk of LDS chunk n * 64 + lane, in bytes from the tile's first row
+  auto source = [&](int n, bool value, int at) {
+    const int L = (wave * kDma + n) * 64 + at, j = L / CH, c = L % CH;
+    const int from = (value ? value_chunk<D>(j, c) : key_chunk<D>(j, c)) - j * CH;  // (a rotation is its own inverse)
+    return (uint32_t)(j * (int)(value ? a.v.ld : a.k.ld) * 2 + from * 16);
+  };
+  constexpr bool kHeld = D < 256;  // (256 dims: computed for each tile, there are no registers to hold them)
+  uint32_t ksrc[kDma], vsrc[kDma];
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int n = 0; n < kDma; n++) {
+      ksrc[n] = source(n, false, lane);
+      vsrc[n] = source(n, true, lane);
+    }
+  }
+  auto request = [&](int t0, int buf) {
+    const __amdgpu_buffer_rsrc_t rk = tile_rsrc<D, BN>(a.k, w, t0), rv = tile_rsrc<D, BN>(a.v, w, t0);
+    uint8_t *to = lds + buf * 2 * kTile + wave * kDma * 1024;
+    const int at = kHeld ? lane : again(lane);
+#pragma unroll
+    for (int n = 0; n < kDma; n++) dma16(rk, kHeld ? ksrc[n] : source(n, false, at), to + n * 1024);
+#pragma unroll
+    for (int n = 0; n < kDma; n++) dma16(rv, kHeld ? vsrc[n] : source(n, true, at), to + kTile + n * 1024);
+  };
+  if (w.keys > 0) request(0, 0);
+
+  u32x4 qf[KC];
+  const int64_t qr = w.q0 + min(row, w.nq - 1);
+#pragma unroll
+  for (int c = 0; c < KC; c++) qf[c] = *(const u32x4 *)((const uint16_t *)a.q.p + qr * a.q.ld + w.h * D + c * 16 + half * 8);
+  // ---- where this lane's operands lie in a tile: the first chunk of a key, and of the values of 16 keys 4 of them for each 4
+  // lanes. The rotation is an exclusive or, so the other chunks are one too (of the low 256 bytes; the rest is an offset).
+  constexpr int KA = D == 64 ? 4 : 8, VA = D == 64 ? 2 : 4;
+  const int kat = key_chunk<D>(col, half) * 16;
+  const int vat = kTile + value_chunk<D>(half * 4 + ((lane & 15) >> 2), ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 +
+                  (lane & 1) * 8;
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; i++)
+#pragma unroll
+    for (int k = 0; k < 16; k++) o[i][k] = 0.f;
+  float mx = kNegInf, l = 0.f;
+  int buf = 0;
+  for (int t0 = 0; t0 < w.keys; t0 += BN, buf ^= 1) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile has arrived
+    __syncthreads();                     // everyone's has, and the other buffer is read
+    if (t0 + BN < w.keys) request(t0 + BN, buf ^ 1);
+    const uint8_t *tile = lds + buf * 2 * kTile;
+    const bool edge = t0 + BN - 1 > all_see;  // some row does not see some key of the tile
+    if (__builtin_expect(edge, 0)) {
+      // a value that is not finite must not reach rows that do not see it as 0 times it: it is cleared and remembered
+      constexpr uint32_t e = F16 ? 0x7C00u : 0x7F80u;
+      bool any = false;
+      u32x4 *vt = (u32x4 *)(lds + buf * 2 * kTile + kTile);
+      for (int i = tid; i < BN * CH; i += 256) {
+        if (t0 + i / CH >= w.nk) vt[i] = u32x4{0u, 0u, 0u, 0u};  // behind the last key
+        const u32x4 y = vt[i];
+#pragma unroll
+        for (int k = 0; k < 4; k++) any |= (y[k] & e) == e || (y[k] >> 16 & e) == e;
+      }
+      if (tid < BN) odd[tid] = 0;
+      if (__syncthreads_or(any)) {
+        for (int i = tid; i < BN * CH; i += 256) {
+          u32x4 y = vt[i];
+          uint32_t all = 0;
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const uint32_t bad = ((y[k] & e) == e ? 0xFFFFu : 0u) | ((y[k] >> 16 & e) == e ? 0xFFFF0000u : 0u);
+            y[k] &= ~bad;
+            all |= bad;
+          }
+          if (all) {
+            vt[i] = y;
+            odd[i / CH] = 1;
+          }
+        }
+        __syncthreads();
+      }
+    }
+    // ---- scores: lane (row col, keys 32 kb + 8 (i / 4) + 4 half + i % 4)
+    const int ka = kHeld ? kat : again(kat), va = kHeld ? vat : again(vat);
+    f32x16 s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int k = 0; k < 16; k++) s[kb][k] = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; c++)
+#pragma unroll
+      for (int kb = 0; kb < KB; kb++) {
+        const u32x4 kf = *(const u32x4 *)(tile + (ka ^ c % KA * 32) + kb * 32 * kRow + c / KA * (KA * 32));
+        s[kb] = mfma32<F16>(kf, qf[c], s[kb]);
+      }
+    float top = kNegInf;
+    if (edge) {
+      const int seen = min(last, w.nk - 1) - t0 - 4 * half;
+#pragma unroll
+      for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (kb * 32 + (i >> 2) * 8 + (i & 3) > seen) s[kb][i] = kNegInf;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
+    top = fmaxf(top, xor_lane<32>(top, lane));
+    const float m1 = fmaxf(mx, top), ms = m1 == kNegInf ? 0.f : m1 * scale;
+    if (__ballot(m1 != mx)) {  // (most tiles change no maximum)
+      const float alpha = m1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f((mx - m1) * scale);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DB; i++) o[i] *= alpha;
+    }
+    mx = m1;
+    float add = 0.f;
+    u32x4 pf[BN / 16];
+#pragma unroll
+    for (int kg = 0; kg < BN / 16; kg++) {
+      f32x8 p;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        p[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kg >> 1][(kg & 1) * 8 + k], scale, -ms));
+        add += p[k];
+      }
+      pf[kg] = F16 ? to_f16x8(p) : to_bf16x8(p);
+    }
+    l += add;
+    // ---- sums
+#pragma unroll
+    for (int kg = 0; kg < BN / 16; kg++)
+#pragma unroll
+      for (int i = 0; i < DB; i++) {
+        // 16 lanes read 4 keys x 16 dims and get 4 keys of one dim each
+        auto tr = [&](int rows) {
+          return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4 *)(tile + (va ^ i % VA * 64) + (kg * 16 + rows) * kRow + i / VA * (VA * 64))));
+        };
+        const u32x2 v0 = tr(0), v1 = tr(8);
+        o[i] = mfma32<F16>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[kg], o[i]);
+      }
+    // ---- rows that see a value that is not finite
+    if (__builtin_expect(edge, 0)) {
+      for (int j = 0; j < min(BN, w.nk - t0); j++) {
+        if (!odd[j] || t0 + j > last) continue;
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+          for (int k = 0; k < 16; k++) {
+            const int64_t at = (int64_t)(w.k0 + t0 + j) * a.v.ld + w.hk * D + i * 32 + (k >> 2) * 8 + half * 4 + (k & 3);
+            const uint32_t v = ((const uint16_t *)a.v.p)[at], e = F16 ? 0x7C00u : 0x7F80u;
+            if ((v & e) == e) o[i][k] = __builtin_nanf("");
+            asm volatile("" ::: "memory");  // (one at a time: this is rare, registers are not)
+          }
+      }
+      __syncthreads();  // `odd` is read
+    }
+  }
+  l += xor_lane<32>(l, lane);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (row < w.nq) {
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int64_t at = (w.q0 + row) * a.out.ld + w.h * D + i * 32 + k * 8 + half * 4;
+        const f32x4 v = {o[i][4 * k] * inv, o[i][4 * k + 1] * inv, o[i][4 * k + 2] * inv, o[i][4 * k + 3] * inv};
+        u32x2 r;
+        if constexpr (F16) {
+          f16x4 x;
+#pragma unroll
+          for (int y = 0; y < 4; y++) x[y] = (_Float16)v[y];
+          r = __builtin_bit_cast(u32x2, x);
+        } else {
+          bf16x4 x;
+#pragma unroll
+          for (int y = 0; y < 4; y++) x[y] = (__bf16)v[y];
+          r = __builtin_bit_cast(u32x2, x);
+        }
+        *(u32x2 *)((uint16_t *)a.out.p + at) = r;
+      }
+  }
+}
+
+// keys of a tile: what three planes of 256 dims leave room for in LDS; 16 bits: what 256 dims leave registers for
 template <int D, int NT>
-constexpr int kBN = D == 256 && NT == 3 ? 32 : 64;
+constexpr int kBN = D == 256 ? 32 : 64;
 
 template <typename F>
 void each(F &&f) {  // every instance: dims, parts, fp16
@@ -303,8 +551,8 @@ void each(F &&f) {  // every instance: dims, parts, fp16
   dims(std::integral_constant<int, 1>(), std::true_type());
 }
 template <int D, int NT>
-constexpr int prompt_lds() {
-  return 2 * NT * kBN<D, NT> * D * 2;
+constexpr int prompt_lds() {  // three parts of keys and values, or two buffers of them
+  return (NT == 3 ? 6 : 4) * kBN<D, NT> * D * 2;
 }
 
 }  // namespace
@@ -315,8 +563,12 @@ void launch_attn_prompt(const PromptArgs &a, hipStream_t s) {
     constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
     constexpr bool F16 = decltype(f16)::value;
     if (a.D == D && a.type == (NT == 3 ? kRowF32 : F16 ? kRowF16 : kRowBf16))
-      hipLaunchKernelGGL((attn_prompt<D, kBN<D, NT>, NT, F16>), dim3((unsigned)(blocks * a.Hq)), dim3(256),
-                         (prompt_lds<D, NT>()), s, a);
+      if constexpr (NT == 3)
+        hipLaunchKernelGGL((attn_prompt<D, kBN<D, NT>, NT, F16>), dim3((unsigned)(blocks * a.Hq)), dim3(256),
+                           (prompt_lds<D, NT>()), s, a);
+      else
+        hipLaunchKernelGGL((attn_prompt16<D, kBN<D, NT>, F16>), dim3((unsigned)(blocks * a.Hq)), dim3(256),
+                           (prompt_lds<D, NT>()), s, a);
   });
   IJ_HIP(hipGetLastError());
 }
@@ -326,8 +578,11 @@ void init_attn_attrs() {
   init_decode_attrs();
   each([&](auto dim, auto nt, auto f16) {
     constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
-    IJ_HIP(hipFuncSetAttribute((const void *)attn_prompt<D, kBN<D, NT>, NT, decltype(f16)::value>,
-                               hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<D, NT>()));
+    constexpr bool F16 = decltype(f16)::value;
+    const void *f;
+    if constexpr (NT == 3) f = (const void *)attn_prompt<D, kBN<D, NT>, NT, F16>;
+    else f = (const void *)attn_prompt16<D, kBN<D, NT>, F16>;
+    IJ_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<D, NT>()));
   });
 }
 
