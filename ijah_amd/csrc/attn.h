@@ -163,10 +163,12 @@ struct PromptArgs {
   int n, Hq, H, D, type, Rq, Rk;
   RowMat q, k, v, out;
   const int *q_rows, *k_rows;
+  int cus;         // compute units of the device
   float scale;     // times log2 e
 };
 void launch_kv_write(const KvArgs &a, hipStream_t s);
 void launch_kv_read(const KvArgs &a, hipStream_t s);
+int compute_units();
 int decode_grid(int D);  // workgroups of the decode kernel: what the chip runs at once
 void launch_attn_decode(const DecArgs &a, hipStream_t s);
 void launch_attn_prompt(const PromptArgs &a, hipStream_t s);

@@ -707,12 +707,16 @@ void each(F &&f) {  // every instance
 
 }  // namespace
 
-int decode_grid(int D) {
-  int dev = 0, cus = 0;
-  IJ_HIP(hipGetDevice(&dev));
-  IJ_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-  return std::min(cus * per_cu(D), kJoin * kJoins);  // (256 CUs on an MI355X)
+int compute_units() {
+  static const int n = [] {
+    int dev = 0, cus = 0;
+    IJ_HIP(hipGetDevice(&dev));
+    IJ_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    return cus;
+  }();
+  return n;
 }
+int decode_grid(int D) { return std::min(compute_units() * per_cu(D), kJoin * kJoins); }  // (256 CUs on an MI355X)
 
 void launch_attn_decode(const DecArgs &a, hipStream_t s) {
   // 16 query rows a block while a token's rows fill no more than that, else 32: each block reads the pages once

@@ -19,6 +19,10 @@ __device__ __forceinline__ int again(int v) {  // v as a value of its own from h
   asm volatile("" : "+v"(v));
   return v;
 }
+__device__ __forceinline__ const void *again(const void *p) {  // the same of a uniform pointer
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // ---- rows: 8 elements from element index i of a row matrix (16-byte aligned) as f32, and back (nearest even)
 // (the type is a template argument: with a run-time one, the compiler dropped the fp16 branch of a copy whose two conversions

@@ -234,7 +234,7 @@ NE_API int ne_attn_prompt(const ne_attn_prompt_desc *d, double *gpu_ms) {
     IJ_CHECK(d->Rq >= 1 && d->Rq <= kMaxRows && d->Rk >= 1 && d->Rk <= kMaxRows, "rows %d and %d (1..%d)", d->Rq, d->Rk,
              kMaxRows);
     IJ_CHECK(d->k_rows || d->Rk == d->Rq, "%d key rows for %d query rows: without k_rows they are the same", d->Rk, d->Rq);
-    IJ_CHECK(((int64_t)d->Rq / 128 + d->n) * d->heads < (1 << 24), "%d rows of %d sequences and %d heads", d->Rq, d->n,
+    IJ_CHECK(((int64_t)d->Rq / 128 + d->n + 1) * d->heads < (1 << 23), "%d rows of %d sequences and %d heads", d->Rq, d->n,
              d->heads);
     check_scale(d->scale);
     ensure_device();
@@ -259,6 +259,7 @@ NE_API int ne_attn_prompt(const ne_attn_prompt_desc *d, double *gpu_ms) {
              (long long)a.k.ld, (long long)a.v.ld);  // (a tile's rows are addressed in 31 bits)
     a.q_rows = ints_of(d->q_rows, (uint64_t)a.n + 1, "q_rows");
     a.k_rows = d->k_rows ? ints_of(d->k_rows, (uint64_t)a.n + 1, "k_rows") : a.q_rows;
+    a.cus = compute_units();
     a.scale = d->scale * kLog2e;
     timed(gpu_ms, [&](hipStream_t st) { launch_attn_prompt(a, st); });
   });

@@ -61,33 +61,86 @@ struct Block {
   int h, hk, nq, nk, i0, off, keys;
   int64_t q0, k0;
 };
-// The last blocks of a sequence see the most keys: they go first. Workgroups go to the XCDs in turn: where the heads divide
+// The blocks that see the most keys go first, so that the short ones fill the chip at the end (up to 64 sequences by their
+// number of blocks, beyond that each sequence's last first). Workgroups go to the XCDs in turn: where the heads divide
 // by their number, an XCD takes an eighth of them, so that the heads of a group read its keys from one L2.
+template <int NT>
 __device__ __forceinline__ bool find_block(const PromptArgs &a, int *sum, Block *w) {
   constexpr int kXcds = 8;
   const int blocks = gridDim.x / a.Hq, id = blockIdx.x;
-  int item;
+  int turn;
   if (a.Hq % kXcds == 0) {
     const int per = a.Hq / kXcds, i = id / kXcds;
     w->h = id % kXcds * per + i % per;
-    item = blocks - 1 - i / per;
+    turn = i / per;
   } else {
     w->h = id % a.Hq;
-    item = blocks - 1 - id / a.Hq;
+    turn = id / a.Hq;
   }
   auto bound = [](const int *p, int b, int R) { return kv_clamp(p[b], 0, R); };
   auto q_of = [&](int b) { return max(bound(a.q_rows, b + 1, a.Rq) - bound(a.q_rows, b, a.Rq), 0); };
   auto items = [&](int i) { return (q_of(i) + kBM - 1) / kBM; };
-  const BatchScan<256> sc = scan_batch<256>(a.n, sum, items);
-  if (item >= sc.total) return false;
-  int before;
-  const int b = find_item<256>(sc, a.n, item, sum, &before, items);
-  w->nq = q_of(b);
-  w->q0 = bound(a.q_rows, b, a.Rq);
-  w->i0 = (item - before) * kBM;
-  const int k0 = bound(a.k_rows, b, a.Rk);
-  w->k0 = k0;
-  w->nk = max(bound(a.k_rows, b + 1, a.Rk) - k0, 0);
+  int b = 0, block;
+  if (a.n <= 64) {
+    // the longest first over all sequences: level by level of blocks from the highest, a sequence a lane
+    const int lane = threadIdx.x & 63, at = min(lane, a.n - 1);
+    const int q0 = bound(a.q_rows, at, a.Rq), nq = max(bound(a.q_rows, at + 1, a.Rq) - q0, 0);
+    const int k0 = bound(a.k_rows, at, a.Rk), nk = max(bound(a.k_rows, at + 1, a.Rk) - k0, 0);
+    const int mine = lane < a.n ? (nq + kBM - 1) / kBM : 0;
+    int top = mine;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) top = max(top, __shfl_xor(top, x));
+    int left = turn;
+    for (block = top - 1; block >= 0; block--) {
+      const uint64_t has = __ballot(mine > block);
+      const int c = __popcll(has);
+      if (left < c) {
+        // the left-th of them
+        const int rank = __popcll(has & ((1ull << lane) - 1));
+        b = (int)__builtin_ctzll(__ballot(mine > block && rank == left) | 1ull << 63);
+        break;
+      }
+      left -= c;
+      if (has & (has - 1)) continue;
+      // one sequence has all the blocks from here on that no other reaches: straight to the next one's level
+      int other = mine > block ? 0 : mine;
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) other = max(other, __shfl_xor(other, x));
+      const int alone = block - other;  // levels below this one that it has alone
+      if (left < alone) {
+        block -= 1 + left;
+        b = (int)__builtin_ctzll(has);
+        break;
+      }
+      left -= alone;
+      block -= alone;
+    }
+    if (block < 0) return false;
+    block = __builtin_amdgcn_readfirstlane(block);
+    b = __builtin_amdgcn_readfirstlane(b);
+    w->nq = __builtin_amdgcn_readlane(nq, b);
+    w->q0 = __builtin_amdgcn_readlane(q0, b);
+    w->nk = __builtin_amdgcn_readlane(nk, b);
+    w->k0 = __builtin_amdgcn_readlane(k0, b);
+  } else {
+    const BatchScan<NT> sc = scan_batch<NT>(a.n, sum, items);
+    const int item = blocks - 1 - turn;
+    if (item >= sc.total) return false;
+    int before;
+    b = find_item<NT>(sc, a.n, item, sum, &before, items);
+    block = item - before;
+    const int k0 = bound(a.k_rows, b, a.Rk);
+    w->nq = q_of(b);
+    w->q0 = bound(a.q_rows, b, a.Rq);
+    w->nk = max(bound(a.k_rows, b + 1, a.Rk) - k0, 0);
+    w->k0 = k0;
+  }
+  // uniform, and known to be
+  w->nq = __builtin_amdgcn_readfirstlane(w->nq);
+  w->q0 = __builtin_amdgcn_readfirstlane((int)w->q0);
+  w->nk = __builtin_amdgcn_readfirstlane(w->nk);
+  w->k0 = __builtin_amdgcn_readfirstlane((int)w->k0);
+  w->i0 = __builtin_amdgcn_readfirstlane(block) * kBM;
   w->off = w->nk - w->nq;
   w->hk = w->h / (a.Hq / a.H);
   w->keys = min(w->nk, min(w->i0 + kBM, w->nq) + w->off);
@@ -100,11 +153,11 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
   constexpr int KC = D / 16, DB = D / 32, KB = BN / 32, CH = D / 8, kPlane = BN * D * 2;
   extern __shared__ __align__(16) uint8_t lds[];  // keys [NT][BN][D], values [NT][BN][D]
   __shared__ int sum[6];
-  __shared__ uint32_t odd[BN];  // keys of the tile whose value is not finite
+  __shared__ uint32_t odd[BN], any;  // keys of the tile whose value is not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5,
             col = lane & 31;
   Block w;
-  if (!find_block(a, sum, &w)) return;
+  if (!find_block<256>(a, sum, &w)) return;
   const int nq = w.nq, nk = w.nk, i0 = w.i0, off = w.off, hk = w.hk, h = w.h, keys = w.keys;
   const int64_t q0 = w.q0, k0 = w.k0;
   const int row = i0 + wave * 32 + col;  // this lane's query row in its sequence
@@ -141,7 +194,8 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
     // ---- the tile into LDS; rows behind the sequence's last key are copies of it. In a tile whose keys not every row
     // sees, a value that is not finite is cleared (0 times it is not 0) and remembered.
     if (edge && tid < BN) odd[tid] = 0;
-    if (edge) __syncthreads();
+    if (tid == 0) any = 0;
+    __syncthreads();
 #pragma unroll 2
     for (int n = 0; n < BN * CH / 256; n++) {
       const int i = n * 256 + tid, j = i / CH, c = i % CH;
@@ -154,7 +208,7 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
           for (int k = 0; k < 8; k++)
             if ((__float_as_uint(y[k]) & 0x7F800000u) == 0x7F800000u) {
               y[k] = 0.f;
-              if (t0 + j < nk) odd[j] = 1;
+              if (t0 + j < nk) odd[j] = any = 1;
             }
         }
 #pragma unroll
@@ -171,7 +225,7 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
           for (int k = 0; k < 4; k++) {
             const uint32_t bad = ((y[k] & e) == e ? 0xFFFFu : 0u) | ((y[k] >> 16 & e) == e ? 0xFFFF0000u : 0u);
             y[k] &= ~bad;
-            if (bad && t0 + j < nk) odd[j] = 1;
+            if (bad && t0 + j < nk) odd[j] = any = 1;
           }
         }
         *(u32x4 *)(lds + key_chunk<D>(j, c) * 16) = x;
@@ -275,7 +329,7 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
       }
     }
     // ---- rows that see a value that is not finite
-    if (edge) {
+    if (edge && any) {
       for (int j = 0; j < min(BN, nk - t0); j++) {
         if (!odd[j] || t0 + j > last) continue;
 #pragma unroll
@@ -323,30 +377,32 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
 // buffer resource ends with the sequence's last key: rows behind it arrive as zeros.
 template <int D, int BN>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const RowMat &m, const Block &w, int t0) {
-  const uint64_t base = (uint64_t)((const uint16_t *)m.p + (w.k0 + t0) * m.ld + w.hk * D);
-  const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)base) |
-                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)) << 32;
-  const int bytes = __builtin_amdgcn_readfirstlane((min(w.nk - t0, BN) - 1) * (int)m.ld * 2 + D * 2);
-  return __builtin_amdgcn_make_buffer_rsrc((void *)u, (short)0, bytes, 0x00020000);
+  const uint16_t *base = (const uint16_t *)m.p + (w.k0 + t0) * m.ld + w.hk * D;
+  return __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (min(w.nk - t0, BN) - 1) * (int)m.ld * 2 + D * 2, 0x00020000);
 }
 
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t at, void *to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)to, 16, at, 0, 0, 0);
 }
 
-template <int D, int BN, bool F16>
-__global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
+//
+// SPLIT 2: where there are fewer blocks than CUs, eight waves take a block, four of them every other tile each, and the two
+// halves' maxima and sums are joined through LDS at the end: a SIMD has two waves then, one's products under the other's
+// exponentials. (All of a block's waves meet at every barrier, so what is decided for both tiles is decided alike.)
+template <int D, int BN, bool F16, int SPLIT>
+__global__ __launch_bounds__(256 * SPLIT, 2) void attn_prompt16(PromptArgs a) {
   constexpr int KC = D / 16, DB = D / 32, KB = BN / 32, CH = D / 8, kTile = BN * D * 2, kRow = D * 2;
   constexpr int kDma = kTile / 1024 / 4;  // of keys, and of values, by each wave
-  extern __shared__ __align__(16) uint8_t lds[];  // two buffers of keys [BN][D], values [BN][D]
-  __shared__ int sum[6];
-  __shared__ uint32_t odd[BN];  // keys of the tile whose value is not finite
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5,
-            col = lane & 31;
+  extern __shared__ __align__(16) uint8_t lds[];  // two buffers of SPLIT times keys [BN][D], values [BN][D]
+  __shared__ int sum[4 * SPLIT + 2];
+  __shared__ uint32_t odds[SPLIT][BN];  // keys of the tiles whose value is not finite
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, stream = SPLIT == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8),
+            wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6 & 3);  // of the stream's four
+  __shared__ float jm[SPLIT][SPLIT == 2 ? 4 : 1][64], jl[SPLIT == 2 ? 4 : 1][64];  // the streams' joins
+  uint32_t *odd = odds[stream];
   Block w;
-  if (!find_block(a, sum, &w)) return;
-  const int row = w.i0 + wave * 32 + col;  // this lane's query row in its sequence
-  const int last = row + w.off;            // the last key it sees
+  if (!find_block<256 * SPLIT>(a, sum, &w)) return;
+  auto row_of = [&](int lane) { return w.i0 + wave * 32 + (lane & 31); };  // a lane's query row in its sequence
   const int all_see = w.i0 + w.off;        // every row of the block sees up to here
   const float scale = a.scale;
 
@@ -367,17 +423,18 @@ __global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
   }
   auto request = [&](int t0, int buf) {
     const __amdgpu_buffer_rsrc_t rk = tile_rsrc<D, BN>(a.k, w, t0), rv = tile_rsrc<D, BN>(a.v, w, t0);
-    uint8_t *to = lds + buf * 2 * kTile + wave * kDma * 1024;
+    uint8_t *to = lds + (buf * SPLIT + stream) * 2 * kTile + wave * kDma * 1024;
     const int at = kHeld ? lane : again(lane);
 #pragma unroll
     for (int n = 0; n < kDma; n++) dma16(rk, kHeld ? ksrc[n] : source(n, false, at), to + n * 1024);
 #pragma unroll
     for (int n = 0; n < kDma; n++) dma16(rv, kHeld ? vsrc[n] : source(n, true, at), to + kTile + n * 1024);
   };
-  if (w.keys > 0) request(0, 0);
+  const int own = stream * BN;  // the stream's tile in a step's SPLIT tiles
+  if (own < w.keys) request(own, 0);
 
   u32x4 qf[KC];
-  const int64_t qr = w.q0 + min(row, w.nq - 1);
+  const int64_t qr = w.q0 + min(row_of(lane), w.nq - 1);
 #pragma unroll
   for (int c = 0; c < KC; c++) qf[c] = *(const u32x4 *)((const uint16_t *)a.q.p + qr * a.q.ld + w.h * D + c * 16 + half * 8);
   // ---- where this lane's operands lie in a tile: the first chunk of a key, and of the values of 16 keys 4 of them for each 4
@@ -387,24 +444,33 @@ __global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
   const int vat = kTile + value_chunk<D>(half * 4 + ((lane & 15) >> 2), ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 +
                   (lane & 1) * 8;
 
+  // A value that is not finite must not reach rows that do not see it, as 0 times it. That takes a look at every value of the
+  // tiles at the edge, so the block is first computed without; only if something in its sums is not finite is it computed
+  // again with such values cleared from those tiles, and made NaN in the rows that do see them.
   f32x16 o[DB];
+  float mx, l;
+  for (bool careful = false;; careful = true) {
 #pragma unroll
   for (int i = 0; i < DB; i++)
 #pragma unroll
     for (int k = 0; k < 16; k++) o[i][k] = 0.f;
-  float mx = kNegInf, l = 0.f;
+  mx = kNegInf;
+  l = 0.f;
   int buf = 0;
-  for (int t0 = 0; t0 < w.keys; t0 += BN, buf ^= 1) {
+  for (int step = 0; step < w.keys; step += SPLIT * BN, buf ^= 1) {
+    const int t0 = step + own;
+    // (the last step may have one tile: the other stream then computes what it finds, no key of which anyone sees)
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile has arrived
     __syncthreads();                     // everyone's has, and the other buffer is read
-    if (t0 + BN < w.keys) request(t0 + BN, buf ^ 1);
-    const uint8_t *tile = lds + buf * 2 * kTile;
-    const bool edge = t0 + BN - 1 > all_see;  // some row does not see some key of the tile
-    if (__builtin_expect(edge, 0)) {
-      // a value that is not finite must not reach rows that do not see it as 0 times it: it is cleared and remembered
+    if (t0 + SPLIT * BN < w.keys) request(t0 + SPLIT * BN, buf ^ 1);
+    uint8_t *tile = lds + (buf * SPLIT + stream) * 2 * kTile;
+    const bool edge = step + SPLIT * BN - 1 > all_see;  // some row does not see some key of the step's tiles
+    bool found = false;  // (the same for all of the workgroup)
+    if (careful && edge) {
       constexpr uint32_t e = F16 ? 0x7C00u : 0x7F80u;
       bool any = false;
-      u32x4 *vt = (u32x4 *)(lds + buf * 2 * kTile + kTile);
+      const int tid = wave * 64 + again(lane);
+      u32x4 *vt = (u32x4 *)(tile + kTile);
       for (int i = tid; i < BN * CH; i += 256) {
         if (t0 + i / CH >= w.nk) vt[i] = u32x4{0u, 0u, 0u, 0u};  // behind the last key
         const u32x4 y = vt[i];
@@ -412,7 +478,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
         for (int k = 0; k < 4; k++) any |= (y[k] & e) == e || (y[k] >> 16 & e) == e;
       }
       if (tid < BN) odd[tid] = 0;
-      if (__syncthreads_or(any)) {
+      found = __syncthreads_or(any) != 0;
+      if (found) {
         for (int i = tid; i < BN * CH; i += 256) {
           u32x4 y = vt[i];
           uint32_t all = 0;
@@ -446,7 +513,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
       }
     float top = kNegInf;
     if (edge) {
-      const int seen = min(last, w.nk - 1) - t0 - 4 * half;
+      const int seen = min(row_of(again(lane)) + w.off, w.nk - 1) - t0 - 4 * half;
 #pragma unroll
       for (int kb = 0; kb < KB; kb++)
 #pragma unroll
@@ -493,15 +560,16 @@ __global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
         o[i] = mfma32<F16>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[kg], o[i]);
       }
     // ---- rows that see a value that is not finite
-    if (__builtin_expect(edge, 0)) {
+    if (__builtin_expect(found, 0)) {
+      const int ln = again(lane), last = row_of(ln) + w.off;  // the last key that the lane's row sees
       for (int j = 0; j < min(BN, w.nk - t0); j++) {
         if (!odd[j] || t0 + j > last) continue;
 #pragma unroll
         for (int i = 0; i < DB; i++)
 #pragma unroll
           for (int k = 0; k < 16; k++) {
-            const int64_t at = (int64_t)(w.k0 + t0 + j) * a.v.ld + w.hk * D + i * 32 + (k >> 2) * 8 + half * 4 + (k & 3);
-            const uint32_t v = ((const uint16_t *)a.v.p)[at], e = F16 ? 0x7C00u : 0x7F80u;
+            const int64_t at = (w.k0 + t0 + j) * a.v.ld + w.hk * D + i * 32 + (k >> 2) * 8 + (again(ln) >> 5) * 4 + (k & 3);
+            const uint32_t v = ((const uint16_t *)again(a.v.p))[at], e = F16 ? 0x7C00u : 0x7F80u;
             if ((v & e) == e) o[i][k] = __builtin_nanf("");
             asm volatile("" ::: "memory");  // (one at a time: this is rare, registers are not)
           }
@@ -509,8 +577,50 @@ __global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
       __syncthreads();  // `odd` is read
     }
   }
+  if (careful) break;
+  uint32_t worst = 0;
+#pragma unroll
+  for (int i = 0; i < DB; i++)
+#pragma unroll
+    for (int k = 0; k < 16; k++) worst = max(worst, __float_as_uint(o[i][k]) & 0x7FFFFFFFu);
+  if (!__syncthreads_or(worst >= 0x7F800000u)) break;
+  int first = own;
+  asm volatile("" : "+s"(first));  // (computed here, not held through the first time)
+  if (own < w.keys) request(first, 0);
+  }
   l += xor_lane<32>(l, lane);
+  if constexpr (SPLIT == 2) {  // the second stream's sums to the first, a register of all lanes at a time
+    jm[stream][wave][lane] = mx;
+    __syncthreads();
+    const float m1 = fmaxf(mx, jm[stream ^ 1][wave][lane]);
+    const float f = mx == kNegInf ? 0.f : __builtin_amdgcn_exp2f((mx - m1) * scale);
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] *= f;
+    f32x4 *js = (f32x4 *)lds + wave * (DB * 4) * 64 + lane;
+    if (stream == 1) {
+#pragma unroll
+      for (int i = 0; i < DB; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) js[(i * 4 + k) * 64] = f32x4{o[i][4 * k], o[i][4 * k + 1], o[i][4 * k + 2], o[i][4 * k + 3]};
+      jl[wave][lane] = l;
+    }
+    __syncthreads();
+    if (stream == 1) return;
+    l += jl[wave][lane];
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const f32x4 v = js[(i * 4 + k) * 64];
+#pragma unroll
+        for (int x = 0; x < 4; x++) o[i][4 * k + x] += v[x];
+        if (k == 3) asm volatile("" : "+v"(o[i]));  // (added here, not where they are stored: registers)
+      }
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int row = row_of(again(lane));
+  const void *to = again(a.out.p);
   if (row < w.nq) {
 #pragma unroll
     for (int i = 0; i < DB; i++)
@@ -530,7 +640,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt16(PromptArgs a) {
           for (int y = 0; y < 4; y++) x[y] = (__bf16)v[y];
           r = __builtin_bit_cast(u32x2, x);
         }
-        *(u32x2 *)((uint16_t *)a.out.p + at) = r;
+        *(u32x2 *)((uint16_t *)to + at) = r;
       }
   }
 }
@@ -550,25 +660,31 @@ void each(F &&f) {  // every instance: dims, parts, fp16
   dims(std::integral_constant<int, 1>(), std::false_type());
   dims(std::integral_constant<int, 1>(), std::true_type());
 }
-template <int D, int NT>
-constexpr int prompt_lds() {  // three parts of keys and values, or two buffers of them
-  return (NT == 3 ? 6 : 4) * kBN<D, NT> * D * 2;
+template <int D, int NT, int SPLIT = 1>
+constexpr int prompt_lds() {  // three parts of keys and values, or two buffers of them for each stream; the join's sums
+  constexpr int tiles = (NT == 3 ? 6 : 4 * SPLIT) * kBN<D, NT> * D * 2, join = SPLIT == 2 ? 4 * (D / 32) * 4 * 1024 : 0;
+  return tiles > join ? tiles : join;
 }
 
 }  // namespace
 
 void launch_attn_prompt(const PromptArgs &a, hipStream_t s) {
-  const int64_t blocks = std::min<int64_t>(a.Rq, a.Rq / kBM + a.n);  // a sequence's last block may be partial
+  const int64_t blocks = std::min<int64_t>(a.Rq, ((int64_t)a.Rq + (int64_t)(kBM - 1) * a.n) / kBM);  // each sequence's last partial
+  // fewer blocks than CUs, and keys enough for two streams of tiles: eight waves a block
+  const bool split = blocks * a.Hq <= a.cus && a.Rk >= 512;
   each([&](auto dim, auto nt, auto f16) {
     constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
     constexpr bool F16 = decltype(f16)::value;
     if (a.D == D && a.type == (NT == 3 ? kRowF32 : F16 ? kRowF16 : kRowBf16))
+    {
+      const dim3 grid((unsigned)(blocks * a.Hq));
       if constexpr (NT == 3)
-        hipLaunchKernelGGL((attn_prompt<D, kBN<D, NT>, NT, F16>), dim3((unsigned)(blocks * a.Hq)), dim3(256),
-                           (prompt_lds<D, NT>()), s, a);
+        hipLaunchKernelGGL((attn_prompt<D, kBN<D, NT>, NT, F16>), grid, dim3(256), (prompt_lds<D, NT>()), s, a);
+      else if (split)
+        hipLaunchKernelGGL((attn_prompt16<D, kBN<D, NT>, F16, 2>), grid, dim3(512), (prompt_lds<D, NT, 2>()), s, a);
       else
-        hipLaunchKernelGGL((attn_prompt16<D, kBN<D, NT>, F16>), dim3((unsigned)(blocks * a.Hq)), dim3(256),
-                           (prompt_lds<D, NT>()), s, a);
+        hipLaunchKernelGGL((attn_prompt16<D, kBN<D, NT>, F16, 1>), grid, dim3(256), (prompt_lds<D, NT>()), s, a);
+    }
   });
   IJ_HIP(hipGetLastError());
 }
@@ -579,10 +695,15 @@ void init_attn_attrs() {
   each([&](auto dim, auto nt, auto f16) {
     constexpr int D = decltype(dim)::value, NT = decltype(nt)::value;
     constexpr bool F16 = decltype(f16)::value;
-    const void *f;
-    if constexpr (NT == 3) f = (const void *)attn_prompt<D, kBN<D, NT>, NT, F16>;
-    else f = (const void *)attn_prompt16<D, kBN<D, NT>, F16>;
-    IJ_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<D, NT>()));
+    auto raise = [](const void *f, int bytes) {
+      IJ_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    };
+    if constexpr (NT == 3) {
+      raise((const void *)attn_prompt<D, kBN<D, NT>, NT, F16>, prompt_lds<D, NT>());
+    } else {
+      raise((const void *)attn_prompt16<D, kBN<D, NT>, F16, 1>, prompt_lds<D, NT>());
+      raise((const void *)attn_prompt16<D, kBN<D, NT>, F16, 2>, prompt_lds<D, NT, 2>());
+    }
   });
 }
 

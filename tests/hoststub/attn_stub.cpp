@@ -29,6 +29,7 @@ void launch_kv_read(const KvArgs &a, hipStream_t) {
   kv = a;
   launches++;
 }
+int compute_units() { return 256; }
 int decode_grid(int) { return 256; }
 void launch_attn_decode(const DecArgs &a, hipStream_t) {
   dec = a;
