@@ -405,6 +405,8 @@ __global__ __launch_bounds__(256 * SPLIT, 2) void attn_prompt16(PromptArgs a) {
   auto row_of = [&](int lane) { return w.i0 + wave * 32 + (lane & 31); };  // a lane's query row in its sequence
   const int all_see = w.i0 + w.off;        // every row of the block sees up to here
   const float scale = a.scale;
+  // the last key that any row of the wave sees; a tile behind it is none of its work
+  const int wave_last = w.i0 + wave * 32 < w.nq ? min(w.i0 + wave * 32 + 31, w.nq - 1) + w.off : -1;
 
   // ---- where this lane's DMAs read: row and chunk of LDS chunk n * 64 + lane, in bytes from the tile's first row
   auto source = [&](int n, bool value, int at) {
@@ -497,6 +499,7 @@ __global__ __launch_bounds__(256 * SPLIT, 2) void attn_prompt16(PromptArgs a) {
         __syncthreads();
       }
     }
+    if (t0 <= wave_last) {
     // ---- scores: lane (row col, keys 32 kb + 8 (i / 4) + 4 half + i % 4)
     const int ka = kHeld ? kat : again(kat), va = kHeld ? vat : again(vat);
     f32x16 s[KB];
@@ -559,6 +562,7 @@ __global__ __launch_bounds__(256 * SPLIT, 2) void attn_prompt16(PromptArgs a) {
         const u32x2 v0 = tr(0), v1 = tr(8);
         o[i] = mfma32<F16>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[kg], o[i]);
       }
+    }
     // ---- rows that see a value that is not finite
     if (__builtin_expect(found, 0)) {
       const int ln = again(lane), last = row_of(ln) + w.off;  // the last key that the lane's row sees

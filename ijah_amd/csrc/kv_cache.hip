@@ -61,45 +61,57 @@ template <int KIND, int D, int TYPE>
 __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
   constexpr int NT = kThreads<D>, kPitch = D * kv_esize(KIND) + 4;  // bytes of a tile row in LDS
   __shared__ int sum[NT / 64 + 2];
-  __shared__ uint32_t amax[2][NT / 64][16];
+  __shared__ uint32_t amax[2][4][NT / 64][16];
   __shared__ __align__(16) uint8_t tile[kKvPage * kPitch];
   const int tid = threadIdx.x, tok = tid & 15, part = tid >> 4, h = blockIdx.y;
   Piece p;
   if (!find_piece<NT>(a.s, (int)blockIdx.x, sum, &p) || p.page < 0) return;
   uint8_t *blk = a.base + ((int64_t)p.page * a.H + h) * kv_block_bytes(KIND, D);
-  for (int g = p.j0 >> 4; g <= (p.j1 - 1) >> 4; g++) {
+  // all of the piece's rows are requested at once: four groups of 16 tokens
+  f32x8 k[4], v[4];
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
     const int j = g * 16 + tok;
-    const bool on = j >= p.j0 && j < p.j1;
-    f32x8 k, v;
-    if (on) {
-      k = load8<TYPE>(a.k, p.row0 + j - p.j0, h * D + part * 8);
-      v = load8<TYPE>(a.v, p.row0 + j - p.j0, h * D + part * 8);
+    if (j >= p.j0 && j < p.j1) {
+      k[g] = load8<TYPE>(a.k, p.row0 + j - p.j0, h * D + part * 8);
+      v[g] = load8<TYPE>(a.v, p.row0 + j - p.j0, h * D + part * 8);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++) k[i] = v[i] = 0.f;
+      for (int i = 0; i < 8; i++) k[g][i] = v[g][i] = 0.f;
     }
-    if constexpr (KIND == kKvI8) {
-      // the largest |x| as its bits: an infinity or a NaN is then larger than any number
+  }
+  if constexpr (KIND == kKvI8) {
+    // the largest |x| as its bits: an infinity or a NaN is then larger than any number
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
       uint32_t mk = 0, mv = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        mk = max(mk, __float_as_uint(k[i]) & 0x7FFFFFFFu);
-        mv = max(mv, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        mk = max(mk, __float_as_uint(k[g][i]) & 0x7FFFFFFFu);
+        mv = max(mv, __float_as_uint(v[g][i]) & 0x7FFFFFFFu);
       }
 #pragma unroll
       for (int x = 16; x < 64; x <<= 1) {
         mk = max(mk, (uint32_t)__shfl_xor((int)mk, x));
         mv = max(mv, (uint32_t)__shfl_xor((int)mv, x));
       }
-      __syncthreads();  // the round before has read its maxima
       if ((tid & 63) < 16) {
-        amax[0][tid >> 6][tok] = mk;
-        amax[1][tid >> 6][tok] = mv;
+        amax[0][g][tid >> 6][tok] = mk;
+        amax[1][g][tid >> 6][tok] = mv;
       }
-      __syncthreads();
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    const int j = g * 16 + tok;
+    const bool on = j >= p.j0 && j < p.j1;
+    if constexpr (KIND == kKvI8) {
+      uint32_t mk = 0, mv = 0;
+#pragma unroll
       for (int w = 0; w < NT / 64; w++) {
-        mk = max(mk, amax[0][w][tok]);
-        mv = max(mv, amax[1][w][tok]);
+        mk = max(mk, amax[0][g][w][tok]);
+        mv = max(mv, amax[1][g][w][tok]);
       }
       auto quant = [](const f32x8 &x, uint32_t m, float *step) {
         const float s = m < 0x7F800000u ? __uint_as_float(m) * (1.f / 127.f) : __builtin_nanf("");
@@ -112,48 +124,58 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
         }
         return o;
       };
-      float ks, vs;
-      const u32x2 kq = quant(k, mk, &ks), vq = quant(v, mv, &vs);
       if (on) {
+        float ks, vs;
+        const u32x2 kq = quant(k[g], mk, &ks), vq = quant(v[g], mv, &vs);
         *(u32x2 *)(blk + kv_key_at(KIND, D, j, part * 8)) = kq;
         if (part == 0) {
           *(float *)(blk + kv_step_at(D, 0, j)) = ks;
           *(float *)(blk + kv_step_at(D, 1, j)) = vs;
         }
+        word *t = (word *)(tile + j * kPitch + part * 8);
+        t[0] = vq[0];
+        t[1] = vq[1];
       }
-      word *t = (word *)(tile + j * kPitch + part * 8);
-      t[0] = vq[0];
-      t[1] = vq[1];
-    } else {
-      const u32x4 kq = KIND == kKvBf16 ? to_bf16x8(k) : to_f16x8(k), vq = KIND == kKvBf16 ? to_bf16x8(v) : to_f16x8(v);
-      if (on) *(u32x4 *)(blk + kv_key_at(KIND, D, j, part * 8)) = kq;
+    } else if (on) {
+      *(u32x4 *)(blk + kv_key_at(KIND, D, j, part * 8)) = KIND == kKvBf16 ? to_bf16x8(k[g]) : to_f16x8(k[g]);
+      const u32x4 vq = KIND == kKvBf16 ? to_bf16x8(v[g]) : to_f16x8(v[g]);
       word *t = (word *)(tile + j * kPitch + part * 16);
 #pragma unroll
       for (int i = 0; i < 4; i++) t[i] = vq[i];
     }
   }
   __syncthreads();
-  // half granules: the 4 keys 16 (kg, half) + 4 quad + {0..3} of one dim
-  constexpr int E = kv_esize(KIND);
-  for (int i = tid; i < (D / 16) * 4 * 64; i += NT) {
-    const int dl = i & 15, quad = (i >> 4) & 3, g = (i >> 6) & 3, d = (i >> 8) * 16 + dl, j = g * 16 + quad * 4;
-    if (j + 4 <= p.j0 || j >= p.j1) continue;
-    uint8_t *to = blk + kv_value_at(KIND, D, j, d);
-    uint32_t e[4];
+  // granules of the values: the keys 4 quad + {0..3} of two groups of 16 (8 bits: of all four) of one dim
+  constexpr int E = kv_esize(KIND), G = E == 2 ? 2 : 4;  // groups of a granule
+  for (int i = tid; i < (D / 16) * (4 / G) * 64; i += NT) {
+    const int dl = i & 15, quad = (i >> 4) & 3, g0 = (i >> 6) % (4 / G) * G, d = (i >> 6) / (4 / G) * 16 + dl;
+    const int first = g0 * 16 + quad * 4, last = first + (G - 1) * 16 + 3;
+    if (last < p.j0 || first >= p.j1) continue;
+    uint8_t *to = blk + kv_value_at(KIND, D, first, d);
+    u32x4 w = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      e[k] = E == 2 ? *(const half_word *)(tile + (j + k) * kPitch + d * 2) : tile[(j + k) * kPitch + d];
-    if (j >= p.j0 && j + 4 <= p.j1) {
-      if constexpr (E == 2) *(u32x2 *)to = u32x2{e[0] | e[1] << 16, e[2] | e[3] << 16};
-      else *(uint32_t *)to = e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24;
-    } else {
+    for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (j + k >= p.j0 && j + k < p.j1) {
-          if constexpr (E == 2) ((uint16_t *)to)[k] = (uint16_t)e[k];
-          else to[k] = (uint8_t)e[k];
-        }
+      for (int n = 0; n < 4; n++) {
+        const int j = first + g * 16 + n, at = (g * 4 + n) * E;  // its byte in the granule
+        const uint32_t e = E == 2 ? *(const half_word *)(tile + j * kPitch + d * 2) : tile[j * kPitch + d];
+        w[at >> 2] |= e << (at & 3) * 8;
+      }
+    if (first >= p.j0 && last < p.j1) {
+      *(u32x4 *)to = w;
+      continue;
     }
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        const int j = first + g * 16 + n, at = (g * 4 + n) * E;
+        if (j >= p.j0 && j < p.j1) {
+          const uint32_t e = w[at >> 2] >> (at & 3) * 8;
+          if constexpr (E == 2) *(uint16_t *)(to + at) = (uint16_t)e;
+          else to[at] = (uint8_t)e;
+        }
+      }
   }
 }
 
@@ -201,33 +223,55 @@ __global__ __launch_bounds__(kThreads<D>) void kv_read(KvArgs a) {
     return;
   }
   const uint8_t *blk = a.base + ((int64_t)p.page * a.H + h) * kv_block_bytes(KIND, D);
-  // values: half granules (4 keys of a dim) into the tile's rows
-  for (int i = tid; i < (D / 16) * 4 * 64; i += NT) {
-    const int dl = i & 15, quad = (i >> 4) & 3, g = (i >> 6) & 3, d = (i >> 8) * 16 + dl, j = g * 16 + quad * 4;
-    if (j + 4 <= p.j0 || j >= p.j1) continue;
-    const uint8_t *from = blk + kv_value_at(KIND, D, j, d);
-    if constexpr (E == 2) {
-      const u32x2 w = *(const u32x2 *)from;
+  // everything is requested at once: the keys' chunks, the steps, the granules of the values
+  constexpr int G = E == 2 ? 2 : 4, VN = (D / 16) * (4 / G) * 64 / NT;  // 16-token groups of a granule; granules of a thread
+  u32x4 kq[4], vq[VN];
+  float ks[4], vs[4];
 #pragma unroll
-      for (int k = 0; k < 4; k++) *(half_word *)(tile + (j + k) * kPitch + d * 2) = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+  for (int g = 0; g < 4; g++) {
+    const int j = g * 16 + tok;
+    if constexpr (KIND == kKvI8) {
+      const u32x2 w = *(const u32x2 *)(blk + kv_key_at(KIND, D, j, part * 8));
+      kq[g] = u32x4{w[0], w[1], 0u, 0u};
+      ks[g] = *(const float *)(blk + kv_step_at(D, 0, j));
+      vs[g] = *(const float *)(blk + kv_step_at(D, 1, j));
     } else {
-      const uint32_t w = *(const uint32_t *)from;
-#pragma unroll
-      for (int k = 0; k < 4; k++) tile[(j + k) * kPitch + d] = (uint8_t)(w >> (8 * k));
+      kq[g] = *(const u32x4 *)(blk + kv_key_at(KIND, D, j, part * 8));
     }
   }
+#pragma unroll
+  for (int n = 0; n < VN; n++) {
+    const int i = n * NT + tid, d = (i >> 6) / (4 / G) * 16 + (i & 15), first = (i >> 6) % (4 / G) * G * 16 + ((i >> 4) & 3) * 4;
+    vq[n] = *(const u32x4 *)(blk + kv_value_at(KIND, D, first, d));
+  }
+  // (what lies outside of the piece is another's or nobody's: it is read, and goes nowhere)
+#pragma unroll
+  for (int n = 0; n < VN; n++) {
+    const int i = n * NT + tid, d = (i >> 6) / (4 / G) * 16 + (i & 15), first = (i >> 6) % (4 / G) * G * 16 + ((i >> 4) & 3) * 4;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const int at = (g * 4 + x) * E;
+        const uint32_t e = vq[n][at >> 2] >> (at & 3) * 8;
+        uint8_t *t = tile + (first + g * 16 + x) * kPitch + d * E;
+        if constexpr (E == 2) *(half_word *)t = (uint16_t)e;
+        else *t = (uint8_t)e;
+      }
+  }
   __syncthreads();
-  for (int g = p.j0 >> 4; g <= (p.j1 - 1) >> 4; g++) {
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
     const int j = g * 16 + tok;
     if (j < p.j0 || j >= p.j1) continue;
     f32x8 k, v;
     if constexpr (KIND == kKvI8) {
-      k = widen8(*(const u32x2 *)(blk + kv_key_at(KIND, D, j, part * 8)), *(const float *)(blk + kv_step_at(D, 0, j)));
       const word *t = (const word *)(tile + j * kPitch + part * 8);
-      v = widen8(u32x2{t[0], t[1]}, *(const float *)(blk + kv_step_at(D, 1, j)));
+      k = widen8(u32x2{kq[g][0], kq[g][1]}, ks[g]);
+      v = widen8(u32x2{t[0], t[1]}, vs[g]);
     } else {
-      k = widen<KIND>(*(const u32x4 *)(blk + kv_key_at(KIND, D, j, part * 8)));
       const word *t = (const word *)(tile + j * kPitch + part * 16);
+      k = widen<KIND>(kq[g]);
       v = widen<KIND>(u32x4{t[0], t[1], t[2], t[3]});
     }
     store8<TYPE>(a.k, p.row0 + j - p.j0, h * D + part * 8, k);
