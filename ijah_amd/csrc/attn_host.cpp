@@ -34,7 +34,7 @@ int row_type(int dtype) {
 }
 void check_dim(int dim) { IJ_CHECK(dim == 64 || dim == 128 || dim == 256, "dim %d (64, 128 or 256)", dim); }
 void check_scale(float s) {
-  IJ_CHECK(s > 0.f && std::isfinite(s), "scale %g (a positive number)", (double)s);
+  IJ_CHECK(s > 0.f && s < 1e38f, "scale %g (a positive number)", (double)s);
 }
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -224,18 +224,25 @@ def plain(q, k, v, seen, scale):
     m, Hq, D = q.shape
     L, H, _ = k.shape
     out, mag, S, vmax = np.zeros((m, Hq, D)), np.zeros((m, Hq, D)), np.zeros((m, Hq, 1)), np.zeros((m, Hq, D))
+    sees = np.arange(L) <= np.asarray(seen)[:, None]
+    some = sees.any(1)
+    if not some.any():
+        return out, mag, S, vmax
+    finite = np.isfinite(k).all() and np.isfinite(v).all()
     for h in range(Hq):
         kh, vh = k[:, h // (Hq // H)], v[:, h // (Hq // H)]
-        for i in range(m):
-            n = min(max(int(seen[i]) + 1, 0), L)
-            if not n:
-                continue
-            s = kh[:n] @ q[i, h] * scale
-            p = np.exp(s - s.max())
-            out[i, h] = p @ vh[:n] / p.sum()
-            mag[i, h] = p @ np.abs(vh[:n]) / p.sum()
-            vmax[i, h] = np.abs(vh[:n]).max(0) / p.sum()
-            S[i, h] = scale * (np.abs(kh[:n]) @ np.abs(q[i, h])).max()
+        rows = np.nonzero(some)[0]
+        for r in np.split(rows, range(256, len(rows), 256)):  # (a few rows at a time; one by one where 0 times a value is not 0)
+            for i in ([r] if finite else r[:, None]):
+                n = L if finite else int(sees[i[0]].sum())
+                on = sees[i][:, :n]
+                s = np.where(on, q[i, h] @ kh[:n].T * scale, -np.inf)
+                p = np.where(on, np.exp(s - s.max(1, keepdims=True)), 0)
+                l = p.sum(1, keepdims=True)
+                out[i, h] = p @ vh[:n] / l
+                mag[i, h] = p @ np.abs(vh[:n]) / l
+                vmax[i, h] = np.abs(vh[:n]).max(0) / l
+                S[i, h] = np.where(on, scale * (np.abs(q[i, h]) @ np.abs(kh[:n]).T), 0).max(1, keepdims=True)
     return out, mag, S, vmax
 
 
@@ -511,6 +518,123 @@ def test_prompt_ranges_f32(eng):
     v *= np.exp(8 * rows_like(rng, n, 1, 1))
     got = eng.attn_prompt(q, k, v, [0, n])
     check(got, plain(q, k, v, np.arange(n), D ** -0.5), n, D, "F32", True)
+
+
+@pytest.mark.parametrize("dtype,Hq,H,D", [("BF16", 64, 8, 64), ("F16", 48, 4, 128), ("BF16", 44, 2, 256)])
+def test_prompt_one_stream(eng, dtype, Hq, H, D):
+    """more blocks than CUs: a workgroup of four waves takes a block's tiles alone"""
+    print(dtype, Hq, D, flush=True)
+    prompt_case(eng, np.random.default_rng(D), [700, 130], [740, 130], Hq, H, D, dtype)
+
+
+@pytest.mark.parametrize("dtype,D", [("F32", 128), ("BF16", 64), ("F16", 128), ("BF16", 256)])
+def test_prompt_two_streams_with_values_that_are_not_finite(eng, dtype, D):
+    """few blocks and many keys: two streams of tiles, the second without a tile in the last step or with; later keys that are
+    not finite change nothing in earlier rows"""
+    print(dtype, D, flush=True)
+    rng = np.random.default_rng(25)
+    for n in (600, 640, 673):
+        q, k, v = rows_like(rng, n, 2, D), rows_like(rng, n, 1, D), rows_like(rng, n, 1, D)
+        (qr, q), (kr, _), (vr, _) = (cast(x, dtype) for x in (q, k, v))
+        r, ob = up(eng, np.array([0, n], np.int32)), eng.alloc(qr.nbytes)
+        eng.attn_prompt_bufs(1, r, None, n, n, 2, 1, D, up(eng, qr), up(eng, kr), up(eng, vr), ob, dtype)
+        clean = values(ob, dtype, (n, 2, D))
+        check(clean, plain(q, cast(k, dtype)[1], cast(v, dtype)[1], np.arange(n), D ** -0.5), n, D, dtype, True, n)
+        at = n - 70
+        v[at, 0, 1], v[at + 40, 0, 2], k[n - 3] = np.inf, np.nan, np.nan
+        (kr, _), (vr, _) = (cast(x, dtype) for x in (k, v))
+        eng.attn_prompt_bufs(1, r, None, n, n, 2, 1, D, up(eng, qr), up(eng, kr), up(eng, vr), ob, dtype)
+        got = values(ob, dtype, (n, 2, D))
+        assert np.array_equal(got[:at], clean[:at])
+        assert not np.isfinite(got[at:, :, 1]).any() and not np.isfinite(got[at + 40:, :, 2]).any()
+        assert np.array_equal(got[at:n - 3, :, 3:], clean[at:n - 3, :, 3:])
+
+
+@pytest.mark.parametrize("n", [64, 65, 130, 256, 257, 700])
+def test_many_sequences(eng, n):
+    """batches around the sizes at which the kernels divide them differently: one lane a sequence, several, all threads"""
+    print(n, flush=True)
+    rng = np.random.default_rng(n)
+    H, Hq, D = 1, 4, 64
+    lens = [int(x) for x in rng.integers(0, 200, n)]
+    new = [min(v, int(x)) for v, x in zip(lens, rng.integers(0, 3, n))]
+    decode_case(eng, rng, lens, new, Hq, H, D, "F16", "F32")  # writes and reads are checked below
+    pool = Pool(rng, [max(v, 1) for v in lens])
+    kv = eng.kv_create(1, pool.pages, H, D, "BF16")
+    T = sum(lens)
+    k = rows_like(rng, T, H, D)
+    seqs = batch(eng, pool.table, lens, offsets(lens))
+    kv.write(0, seqs, k, -k)
+    got = kv.read(0, seqs, T)
+    assert np.array_equal(got[0], held(k, "BF16")) and np.array_equal(got[1], -held(k, "BF16"))
+    prompt_case(eng, rng, new, lens, Hq, H, D, "BF16")
+    prompt_case(eng, rng, [v % 37 for v in lens], [v % 41 for v in lens], Hq, H, D, "F32")
+
+
+def test_offsets_past_32_bits(eng):
+    """pages beyond 4 GB of the cache, in its last layer, and rows beyond 4 GB of a prompt's keys"""
+    rng = np.random.default_rng(41)
+    H, Hq, D, L = 4, 8, 128, 200
+    kv = eng.kv_create(2, 40000, H, D, "BF16")  # 5.2 GB a layer
+    assert kv.nbytes > 2 * (1 << 32)
+    k, v = rows_like(rng, L, H, D), rows_like(rng, L, H, D)
+    table = np.array([[39999, 33333, 39000, 2]], np.int32)
+    whole = batch(eng, table, [L], [0, L])
+    kv.write(1, whole, k, v)
+    got = kv.read(1, whole, L)
+    assert np.array_equal(got[0], held(k, "BF16")) and np.array_equal(got[1], held(v, "BF16"))
+    assert not kv.read(0, whole, L)[0].any()
+    q = rows_like(rng, 1, Hq, D)
+    check(kv.attend(1, batch(eng, table, [L]), q), plain(q, held(k, "BF16"), held(v, "BF16"), [L - 1], D ** -0.5), L, D, "F32",
+          False)
+    kv.free()
+    n, ld = 1100, 1 << 21  # rows of 4 MB
+    (qr, q), (kr, k), (vr, v) = (cast(rows_like(rng, n, 1, D), "BF16") for _ in range(3))
+    kb = eng.alloc(n * ld * 2)
+    for r in range(n):
+        kb.upload(kr[r], offset=r * ld * 2)
+        kb.upload(vr[r], offset=r * ld * 2 + 1024)
+    ob, rows = eng.alloc(qr.nbytes), up(eng, np.array([0, n], np.int32))
+    eng.attn_prompt_bufs(1, rows, None, n, n, 1, 1, D, up(eng, qr), kb, kb, ob, "BF16", v_off=1024, ldk=ld, ldv=ld)
+    check(values(ob, "BF16", (n, 1, D)), plain(q, k, v, np.arange(n), D ** -0.5), n, D, "BF16", True)
+
+
+def test_two_graphs_of_one_cache(eng):
+    """two captured decode calls over one cache (and its workspace) replayed in turn, with an eager call in between"""
+    hip = hip_runtime()
+    rng = np.random.default_rng(42)
+    H, Hq, D = 2, 16, 128
+    lens = [6000, 900]
+    pool = Pool(rng, lens)
+    kv = eng.kv_create(1, pool.pages, H, D, "BF16")
+    k, v = rows_like(rng, sum(lens), H, D), rows_like(rng, sum(lens), H, D)
+    kv.write(0, batch(eng, pool.table, lens, offsets(lens)), k, v)
+    qs = [up(eng, rows_like(rng, 2, Hq, D)) for _ in range(2)]
+    outs = [eng.alloc(2 * Hq * D * 4) for _ in range(3)]
+    seqs = batch(eng, pool.table, lens)
+    want = []
+    for q in qs:
+        kv.attend_bufs(0, seqs, 2, Hq, q, outs[2])
+        want.append(outs[2].download(np.uint32))
+    s, graphs = eng.lib.ne_stream(), []
+    for q, o in zip(qs, outs):
+        g, ex = C.c_void_p(), C.c_void_p()
+        assert hip.hipStreamBeginCapture(s, 1) == 0
+        kv.attend_bufs(0, seqs, 2, Hq, q, o)
+        assert hip.hipStreamEndCapture(s, C.byref(g)) == 0
+        assert hip.hipGraphInstantiate(C.byref(ex), g, None, None, 0) == 0
+        graphs.append((g, ex))
+    for i in range(6):
+        assert hip.hipGraphLaunch(graphs[i % 2][1], s) == 0
+        if i % 3 == 0:
+            kv.attend_bufs(0, seqs, 2, Hq, qs[0], outs[2])
+        assert hip.hipGraphLaunch(graphs[1 - i % 2][1], s) == 0
+        assert hip.hipStreamSynchronize(s) == 0
+        for o, w in zip(outs, want):
+            assert np.array_equal(o.download(np.uint32), w), i
+    for g, ex in graphs:
+        hip.hipGraphExecDestroy(ex)
+        hip.hipGraphDestroy(g)
 
 
 # ---------------------------------------------------------------------------------------------------- together
