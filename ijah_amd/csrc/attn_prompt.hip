@@ -275,9 +275,15 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
         top = fmaxf(top, s[kb][i]);
       }
     top = fmaxf(top, xor_lane<32>(top, lane));
-    const float m1 = fmaxf(mx, top), ms = m1 == kNegInf ? 0.f : m1 * a.scale;
-    const float alpha = __builtin_amdgcn_exp2f(mx == kNegInf ? kNegInf : __builtin_fmaf(mx, a.scale, -ms));
-    mx = m1;
+    // the maximum that the weights are relative to moves, and the sums with it, only where a weight would pass 2^8
+    if (__ballot((top - mx) * a.scale > 8.f)) {
+      const float m1 = fmaxf(mx, top), alpha = m1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f((mx - m1) * a.scale);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DB; i++) o[i] *= alpha;
+      mx = m1;
+    }
+    const float ms = mx == kNegInf ? 0.f : mx * a.scale;
     float add = 0.f;
 #pragma unroll
     for (int kb = 0; kb < KB; kb++)
@@ -287,9 +293,7 @@ __global__ __launch_bounds__(256) void attn_prompt(PromptArgs a) {
         add += e;
         s[kb][i] = e;
       }
-    l = __builtin_fmaf(l, alpha, add);
-#pragma unroll
-    for (int i = 0; i < DB; i++) o[i] *= alpha;
+    l += add;
     // ---- sums
 #pragma unroll
     for (int kg = 0; kg < BN / 16; kg++) {
@@ -408,29 +412,25 @@ __global__ __launch_bounds__(256 * SPLIT, 2) void attn_prompt16(PromptArgs a) {
   // the last key that any row of the wave sees; a tile behind it is none of its work
   const int wave_last = w.i0 + wave * 32 < w.nq ? min(w.i0 + wave * 32 + 31, w.nq - 1) + w.off : -1;
 
-  // ---- where this lane's DMAs read: row and chunk of LDS chunk n * 64 + lane, in bytes from the tile's first row
-  auto source = [&](int n, bool value, int at) {
-    const int L = (wave * kDma + n) * 64 + at, j = L / CH, c = L % CH;
-    const int from = (value ? value_chunk<D>(j, c) : key_chunk<D>(j, c)) - j * CH;  // (a rotation is its own inverse)
-    return (uint32_t)(j * (int)(value ? a.v.ld : a.k.ld) * 2 + from * 16);
-  };
-  constexpr bool kHeld = D < 256;  // (256 dims: computed for each tile, there are no registers to hold them)
-  uint32_t ksrc[kDma], vsrc[kDma];
-  if constexpr (kHeld) {
-#pragma unroll
-    for (int n = 0; n < kDma; n++) {
-      ksrc[n] = source(n, false, lane);
-      vsrc[n] = source(n, true, lane);
-    }
-  }
+  // ---- where this lane's DMAs read: row and chunk of LDS chunk (wave * kDma + n) * 64 + lane, in bytes from the tile's first
+  // row. The rotation of a row is an exclusive or with a value of the row's number (its own inverse), and the rows of n are a
+  // constant apart, so one row offset and one chunk each serve all n.
+  constexpr int kStep = 64 / CH;  // rows of a DMA
   auto request = [&](int t0, int buf) {
     const __amdgpu_buffer_rsrc_t rk = tile_rsrc<D, BN>(a.k, w, t0), rv = tile_rsrc<D, BN>(a.v, w, t0);
     uint8_t *to = lds + (buf * SPLIT + stream) * 2 * kTile + wave * kDma * 1024;
-    const int at = kHeld ? lane : again(lane);
+    const int at = D == 256 ? again(lane) : lane;  // (256 dims: computed for each tile, there are no registers to hold them)
+    const int srow = wave * kDma * kStep + at / CH, schunk = at % CH;
+    const uint32_t krow = (uint32_t)(srow * (int)a.k.ld * 2), vrow = (uint32_t)(srow * (int)a.v.ld * 2);
+    const uint32_t kchunk = (uint32_t)(key_chunk<D>(srow, schunk) - srow * CH) * 16,
+                   vchunk = (uint32_t)(value_chunk<D>(srow, schunk) - srow * CH) * 16;
 #pragma unroll
-    for (int n = 0; n < kDma; n++) dma16(rk, kHeld ? ksrc[n] : source(n, false, at), to + n * 1024);
+    for (int n = 0; n < kDma; n++)
+      dma16(rk, krow + n * kStep * (uint32_t)a.k.ld * 2 + (kchunk ^ key_chunk<D>(n * kStep, 0) % CH * 16), to + n * 1024);
 #pragma unroll
-    for (int n = 0; n < kDma; n++) dma16(rv, kHeld ? vsrc[n] : source(n, true, at), to + kTile + n * 1024);
+    for (int n = 0; n < kDma; n++)
+      dma16(rv, vrow + n * kStep * (uint32_t)a.v.ld * 2 + (vchunk ^ value_chunk<D>(n * kStep, 0) % CH * 16),
+            to + kTile + n * 1024);
   };
   const int own = stream * BN;  // the stream's tile in a step's SPLIT tiles
   if (own < w.keys) request(own, 0);
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256 * SPLIT, 2) void attn_prompt16(PromptArgs a) {
     }
     if (t0 <= wave_last) {
     // ---- scores: lane (row col, keys 32 kb + 8 (i / 4) + 4 half + i % 4)
-    const int ka = kHeld ? kat : again(kat), va = kHeld ? vat : again(vat);
+    const int ka = again(kat), va = again(vat);  // (the chunks' addresses are computed for each tile: registers)
     f32x16 s[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; kb++)
@@ -528,14 +528,15 @@ __global__ __launch_bounds__(256 * SPLIT, 2) void attn_prompt16(PromptArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, s[kb][i]);
     top = fmaxf(top, xor_lane<32>(top, lane));
-    const float m1 = fmaxf(mx, top), ms = m1 == kNegInf ? 0.f : m1 * scale;
-    if (__ballot(m1 != mx)) {  // (most tiles change no maximum)
-      const float alpha = m1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f((mx - m1) * scale);
+    // the maximum that the weights are relative to moves, and the sums with it, only where a weight would pass 2^8
+    if (__ballot((top - mx) * scale > 8.f)) {
+      const float m1 = fmaxf(mx, top), alpha = m1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f((mx - m1) * scale);
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < DB; i++) o[i] *= alpha;
+      mx = m1;
     }
-    mx = m1;
+    const float ms = mx == kNegInf ? 0.f : mx * scale;
     float add = 0.f;
     u32x4 pf[BN / 16];
 #pragma unroll
