@@ -146,6 +146,9 @@ struct KvArgs {
   RowMat k, v;     // read: written to
   int type;
 };
+struct DecJoin {  // a group whose parts a launch of its own joins (parts 0: none), by its first workgroup
+  int parts, r0, h, row0, nrows;
+};
 struct DecArgs {
   const uint8_t *base;
   int kind, D, H, Hq;
@@ -155,6 +158,8 @@ struct DecArgs {
   float scale;     // times log2 e
   float *part;     // [2 W] slots of dec_slot_floats
   uint32_t *cnt;   // [3 W], zero between launches: by slot of a join's first part, then by first workgroup of a group
+  DecJoin *joins;  // [W]
+  int apart;       // the joins of chunks take a launch of their own
   int W;
 };
 constexpr int kDecRows = 64;  // query rows of a group at most (the partial slots' size)

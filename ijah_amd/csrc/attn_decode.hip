@@ -82,6 +82,30 @@ __device__ __forceinline__ void part_store(__amdgpu_buffer_rsrc_t r, uint32_t at
   __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, (int)at, 0, 16);
 }
 
+// four output elements: dims d .. of the row-th of a sequence's rows of key head h (token, then query head)
+template <int D>
+__device__ __forceinline__ void store4(const DecArgs &a, int r0, int h, int row, int d, f32x4 v) {
+  const int group = a.Hq / a.H, t = row / group;
+  const int64_t at = (r0 + t) * a.out.ld + (h * group + row - t * group) * D + d;
+  if (a.type == kRowF32) {
+    *(f32x4 *)((float *)a.out.p + at) = v;
+    return;
+  }
+  u32x2 w;
+  if (a.type == kRowBf16) {
+    bf16x4 o4;
+#pragma unroll
+    for (int k = 0; k < 4; k++) o4[k] = (__bf16)v[k];
+    w = __builtin_bit_cast(u32x2, o4);
+  } else {
+    f16x4 o4;
+#pragma unroll
+    for (int k = 0; k < 4; k++) o4[k] = (_Float16)v[k];
+    w = __builtin_bit_cast(u32x2, o4);
+  }
+  *(u32x2 *)((uint16_t *)a.out.p + at) = w;
+}
+
 // the place of a segment in the batch
 struct Group {
   int b, h, rb;  // sequence, key head, which of the sequence's row groups
@@ -122,6 +146,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
                                 : load8<kRowF16>(a.q, row, c);
   };
   // ---- the share
+  if (a.apart && tid == 0) a.joins[me].parts = 0;
   auto seq_of = [&](int b) { return dec_seq(kv_seq(a.s, b), group, BR, NB); };
   bool aligned = false;
   int C = 0, chunk = 0, share = 0, u_hi = 0, u = 0;
@@ -153,7 +178,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
       // chunks of up to four pages a wave more than an equal share, if the groups then fit the workgroups: a second segment
       // (its first loads, its join) costs a workgroup about as much as three more pages for each wave
       if (groups <= W) {
-        C = max((share + NW - 1) / NW, RT == 1 ? 1 : 4) * NW;  // (many rows: a join costs more than the pages of a turn)
+        C = max((share + NW - 1) / NW, RT == 1 ? 1 : 2) * NW;  // (many rows: a part costs about as much as a page)
         for (int t = 0; t < 4 && !aligned; t++, C += aligned ? 0 : NW) {
           int m = 0;
 #pragma unroll
@@ -526,6 +551,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
           for (int k = 0; k < 4; k++) o[t][i][k] = __builtin_amdgcn_ldexpf(o[t][i][k], ve);
     }
     // ---- the segment's waves joined
+    const int tj = again(tid);  // (what follows from it is computed here, not held through the pages)
     const int used = max(min(step, pg1 - pg0), 1);  // waves of a block that had a page; one has the zeros of none
     __syncthreads();  // every wave has read its query parts
 #pragma unroll
@@ -546,28 +572,8 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
     const int slot = dec_slot(part, me - part.first) * SLOT;  // in floats
     constexpr int ROWS = NB * BR;
     const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)(2u * W * SLOT * 4), 0x00020000);
-    auto out4 = [&](int m, int d, f32x4 v) {  // four output elements
-      const int row = row0 + m, t = row / group;
-      const int64_t at = (g.q.r0 + t) * a.out.ld + (g.h * group + row - t * group) * D + d;
-      if (a.type == kRowF32) {
-        *(f32x4 *)((float *)a.out.p + at) = v;
-      } else {
-        u32x2 w;
-        if (a.type == kRowBf16) {
-          bf16x4 o4;
-#pragma unroll
-          for (int k = 0; k < 4; k++) o4[k] = (__bf16)v[k];
-          w = __builtin_bit_cast(u32x2, o4);
-        } else {
-          f16x4 o4;
-#pragma unroll
-          for (int k = 0; k < 4; k++) o4[k] = (_Float16)v[k];
-          w = __builtin_bit_cast(u32x2, o4);
-        }
-        *(u32x2 *)((uint16_t *)a.out.p + at) = w;
-      }
-    };
-    for (int i = tid; i < nrows * (D / 4); i += NT) {
+    auto out4 = [&](int m, int d, f32x4 v) { store4<D>(a, g.q.r0, g.h, row0 + m, d, v); };
+    for (int i = tj; i < nrows * (D / 4); i += NT) {
       const int m = i / (D / 4), d = i % (D / 4) * 4;
       const int w0 = m / BR, mm = m - w0 * BR;  // the waves w0, w0 + nb, .. hold the row
       float top = kNegInf, s = 0.f;
@@ -589,11 +595,13 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         out4(m, d, v * (s == 0.f ? 0.f : 1.f / s));
       }
     }
-    // ---- the group's shares joined: parts by kJoin, then their joins
-    if (part.parts > 1) {
+    // ---- the group's shares joined: parts by kJoin, then their joins; or by a launch of its own, that is told which
+    if (aligned && a.apart) {
+      if (part.parts > 1 && chunk == 0 && tj == 0) a.joins[me] = DecJoin{part.parts, g.q.r0, g.h, row0, nrows};
+    } else if (part.parts > 1) {
       // parts k0, k0 + every, .. (cnt of them) into part k0's slot, or into the output
       auto join = [&](int k0, int every, int cnt, bool final) {
-        for (int i = tid; i < cnt * ROWS; i += NT) {
+        for (int i = tj; i < cnt * ROWS; i += NT) {
           const int k = i / ROWS, m = i % ROWS;
           if (m < nrows) {
             const float *sl = a.part + dec_slot(part, k0 + k * every) * SLOT + ROWS * D;
@@ -602,20 +610,20 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
           }
         }
         __syncthreads();
-        if (tid < nrows) {  // each part's factor in place of its maximum, the row's maximum and sum
+        if (tj < nrows) {  // each part's factor in place of its maximum, the row's maximum and sum
           float top = kNegInf, sum = 0.f;
-          for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][tid]);
+          for (int k = 0; k < cnt; k++) top = fmaxf(top, pm[k][tj]);
           const float ms = top == kNegInf ? 0.f : top;
           for (int k = 0; k < cnt; k++) {
-            const float f = __builtin_amdgcn_exp2f(pm[k][tid] - ms);
-            pm[k][tid] = f;
-            sum = __builtin_fmaf(pl[k][tid], f, sum);
+            const float f = __builtin_amdgcn_exp2f(pm[k][tj] - ms);
+            pm[k][tj] = f;
+            sum = __builtin_fmaf(pl[k][tj], f, sum);
           }
           if (!final) {
-            st_cg(a.part + dec_slot(part, k0) * SLOT + ROWS * D + tid, top);
-            st_cg(a.part + dec_slot(part, k0) * SLOT + ROWS * D + ROWS + tid, sum);
+            st_cg(a.part + dec_slot(part, k0) * SLOT + ROWS * D + tj, top);
+            st_cg(a.part + dec_slot(part, k0) * SLOT + ROWS * D + ROWS + tj, sum);
           }
-          pl[0][tid] = sum == 0.f ? 0.f : 1.f / sum;
+          pl[0][tj] = sum == 0.f ? 0.f : 1.f / sum;
         }
         __syncthreads();
         // four dims of a row at a time, kJoin parts' requests in flight and the next ones behind them
@@ -627,7 +635,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
             if (r + k < cnt) in[k] = part_load(parts, (uint32_t)(dec_slot(part, k0 + (r + k) * every) * SLOT + m * D + d) * 4u);
         };
         f32x4 in[kJoin] = {}, next[kJoin] = {}, v = {0.f, 0.f, 0.f, 0.f};
-        int i = tid, r = 0;
+        int i = tj, r = 0;
         if (i < items) request(in, i, 0);
         while (i < items) {
           const bool done = r + kJoin >= cnt;  // the item's last round
@@ -651,7 +659,7 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
       auto last_of = [&](uint32_t *c, int n) {  // every wave's stores have arrived; true in the n-th workgroup to come here
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
-        if (tid == 0) {
+        if (tj == 0) {
           flag = atomicAdd(c, 1u) == (uint32_t)n - 1u;
           if (flag) st_cg(c, 0u);
         }
@@ -683,6 +691,58 @@ __global__ __launch_bounds__(NT, per_cu(D)) void attn_decode(DecArgs a) {
         } while (!g.d.blocks);
       }
     }
+  }
+}
+
+// The parts of the groups that the decode kernel names (rows of several drafts: a part is up to 64 rows, and one workgroup reads
+// 40 GB/s of them). Workgroup (the group's first one, 16 rows of it): the rows' factors in LDS, then four dims a thread, kJoin
+// parts' loads in flight.
+constexpr int kJoinRows = 16;
+template <int D>
+__global__ __launch_bounds__(256) void attn_join(DecArgs a) {
+  constexpr int ROWS = kDecRows, SLOT = dec_slot_floats(D);
+  __shared__ float f[kJoin * kJoins][kJoinRows], inv[kJoinRows];
+  const DecJoin j = a.joins[blockIdx.x];
+  const int m0 = blockIdx.y * kJoinRows, rows = min(j.nrows - m0, kJoinRows), tid = threadIdx.x;
+  if (j.parts == 0 || rows <= 0) return;
+  const float *base = a.part + (int64_t)blockIdx.x * 2 * SLOT;  // part k's slot: 2 k slots on
+  float *sums = inv;
+  for (int i = tid; i < j.parts * kJoinRows; i += 256) {
+    const int k = i / kJoinRows, m = i % kJoinRows;
+    if (m < rows) f[k][m] = base[(int64_t)k * 2 * SLOT + ROWS * D + m0 + m];
+  }
+  __syncthreads();
+  // 16 threads a row
+  const int row = tid >> 4, part = tid & 15;
+  if (row < rows) {
+    float top = kNegInf, sum = 0.f;
+    for (int k = part; k < j.parts; k += 16) top = fmaxf(top, f[k][row]);
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float ms = top == kNegInf ? 0.f : top;
+    for (int k = part; k < j.parts; k += 16) {
+      const float e = __builtin_amdgcn_exp2f(f[k][row] - ms);
+      f[k][row] = e;
+      sum = __builtin_fmaf(base[(int64_t)k * 2 * SLOT + ROWS * D + ROWS + m0 + row], e, sum);
+    }
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor(sum, x);
+    if (part == 0) sums[row] = sum == 0.f ? 0.f : 1.f / sum;
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * (D / 4); i += 256) {
+    const int m = i / (D / 4), d = i % (D / 4) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < j.parts; r += kJoin) {
+      f32x4 in[kJoin];
+#pragma unroll
+      for (int k = 0; k < kJoin; k++)
+        if (r + k < j.parts) in[k] = *(const f32x4 *)(base + (int64_t)(r + k) * 2 * SLOT + (m0 + m) * D + d);
+#pragma unroll
+      for (int k = 0; k < kJoin; k++)
+        if (r + k < j.parts) v += in[k] * f[r + k][m];
+    }
+    store4<D>(a, j.r0, j.h, j.row0 + m0 + m, d, v * inv[m]);
   }
 }
 
@@ -721,15 +781,23 @@ int compute_units() {
 }
 int decode_grid(int D) { return std::min(compute_units() * per_cu(D), kJoin * kJoins); }  // (256 CUs on an MI355X)
 
-void launch_attn_decode(const DecArgs &a, hipStream_t s) {
+void launch_attn_decode(const DecArgs &args, hipStream_t s) {
+  DecArgs a = args;
   // 16 query rows a block while a token's rows fill no more than that, else 32: each block reads the pages once
   const int rt = a.Hq / a.H <= 16 && a.s.R <= a.s.n ? 1 : 2;
+  // many rows that may lie in several chunks (of at least two pages a wave): their joins take a launch of their own
+  a.apart = rt == 2 && (int64_t)a.s.ldt * 2 > 2 * NW;
   each([&](auto kind, auto dim, auto tiles) {
-    if (a.kind == kind && a.D == dim && rt == tiles)
-      hipLaunchKernelGGL((attn_decode<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>), dim3(a.W),
-                         dim3(NT),
-                         (lds_bytes<decltype(kind)::value, decltype(dim)::value, decltype(tiles)::value>()), s, a);
+    constexpr int K = decltype(kind)::value, D = decltype(dim)::value, RT = decltype(tiles)::value;
+    if (a.kind == K && a.D == D && rt == RT)
+      hipLaunchKernelGGL((attn_decode<K, D, RT>), dim3(a.W), dim3(NT), (lds_bytes<K, D, RT>()), s, a);
   });
+  IJ_HIP(hipGetLastError());
+  if (!a.apart) return;
+  const dim3 grid(a.W, kDecRows / kJoinRows);
+  if (a.D == 64) hipLaunchKernelGGL(attn_join<64>, grid, dim3(256), 0, s, a);
+  else if (a.D == 128) hipLaunchKernelGGL(attn_join<128>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(attn_join<256>, grid, dim3(256), 0, s, a);
   IJ_HIP(hipGetLastError());
 }
 

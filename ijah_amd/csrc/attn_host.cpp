@@ -18,8 +18,9 @@ struct ne_kv {
   uint8_t *base = nullptr;
   float *part = nullptr;    // decode: the partial slots of W workgroups
   uint32_t *cnt = nullptr;  // decode: 3 W counters, zero between launches
+  DecJoin *joins = nullptr; // decode: [W]
   ~ne_kv() {
-    for (void *p : {(void *)base, (void *)part, (void *)cnt})
+    for (void *p : {(void *)base, (void *)part, (void *)cnt, (void *)joins})
       if (p) (void)hipFree(p);
   }
 };
@@ -160,6 +161,7 @@ NE_API ne_kv *ne_kv_create(const ne_kv_desc *d) {
     alloc(kv->base, kv->layer_bytes * (uint64_t)d->layers);
     alloc(kv->part, (uint64_t)2 * kv->W * dec_slot_floats(d->dim) * 4);
     alloc(kv->cnt, (uint64_t)3 * kv->W * 4);
+    alloc(kv->joins, (uint64_t)kv->W * sizeof(DecJoin));
     IJ_HIP(hipDeviceSynchronize());
     h = kv.release();
   });
@@ -219,6 +221,8 @@ NE_API int ne_attn_decode(ne_kv *kv, int layer, const ne_kv_seqs *s, int R, int 
     a.scale = scale * kLog2e;
     a.part = kv->part;
     a.cnt = kv->cnt;
+    a.joins = kv->joins;
+    a.apart = 0;
     a.W = kv->W;
     timed(gpu_ms, [&](hipStream_t st) { launch_attn_decode(a, st); });
   });
