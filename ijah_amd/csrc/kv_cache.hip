@@ -57,6 +57,19 @@ __device__ __forceinline__ bool find_piece(const KvSeqs &s, int item, int *sum, 
   return true;
 }
 
+// 8 of a row's elements in steps of its largest magnitude (as bits: an infinity or a NaN is larger than any number) / 127
+__device__ __forceinline__ u32x2 quantise(const f32x8 &x, uint32_t m, float *step) {
+  const float s = m < 0x7F800000u ? __uint_as_float(m) * (1.f / 127.f) : __builtin_nanf("");
+  *step = s;
+  u32x2 o = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float c = s > 0.f ? fminf(fmaxf(rintf(x[i] / s), -127.f), 127.f) : 0.f;
+    o[i >> 2] |= ((uint32_t)(int)c & 0xFFu) << (8 * (i & 3));
+  }
+  return o;
+}
+
 template <int KIND, int D, int TYPE>
 __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
   constexpr int NT = kThreads<D>, kPitch = D * kv_esize(KIND) + 4;  // bytes of a tile row in LDS
@@ -113,20 +126,9 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
         mk = max(mk, amax[0][g][w][tok]);
         mv = max(mv, amax[1][g][w][tok]);
       }
-      auto quant = [](const f32x8 &x, uint32_t m, float *step) {
-        const float s = m < 0x7F800000u ? __uint_as_float(m) * (1.f / 127.f) : __builtin_nanf("");
-        *step = s;
-        u32x2 o = {0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float c = s > 0.f ? fminf(fmaxf(rintf(x[i] / s), -127.f), 127.f) : 0.f;
-          o[i >> 2] |= ((uint32_t)(int)c & 0xFFu) << (8 * (i & 3));
-        }
-        return o;
-      };
       if (on) {
         float ks, vs;
-        const u32x2 kq = quant(k[g], mk, &ks), vq = quant(v[g], mv, &vs);
+        const u32x2 kq = quantise(k[g], mk, &ks), vq = quantise(v[g], mv, &vs);
         *(u32x2 *)(blk + kv_key_at(KIND, D, j, part * 8)) = kq;
         if (part == 0) {
           *(float *)(blk + kv_step_at(D, 0, j)) = ks;
@@ -176,6 +178,62 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
           else to[at] = (uint8_t)e;
         }
       }
+  }
+}
+
+// Few rows of each sequence (a decode step, drafts): a wave takes one row and as many heads as it has lanes for, 8 dims a lane.
+// The row's sequence by bisection of the row table (uniform, through the scalar cache); nothing is shared, so there is no LDS
+// and no barrier, and a value's dims are stored one by one, 16 bytes apart.
+template <int KIND, int D, int TYPE>
+__global__ __launch_bounds__(256) void kv_write_rows(KvArgs a) {
+  constexpr int kParts = D / 8, kHeads = 64 / kParts;
+  const int lane = threadIdx.x & 63, part = lane % kParts;
+  const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int h = blockIdx.y * kHeads + lane / kParts;
+  if (row >= a.s.R || (!a.s.rows && row >= a.s.n)) return;
+  int b = row;
+  if (a.s.rows) {  // the last sequence that begins at or before the row
+    b = 0;
+    for (int lo = 1, hi = a.s.n; lo < hi;) {
+      const int mid = (lo + hi) >> 1;
+      if (a.s.rows[mid] <= row) b = mid, lo = mid + 1;
+      else hi = mid;
+    }
+  }
+  const KvSeq q = kv_seq(a.s, b);
+  const int p = q.len - q.nr + row - q.r0;  // the row's token
+  if (row < q.r0 || row >= q.r0 + q.nr || p < 0) return;
+  const int id = a.s.table[(int64_t)b * a.s.ldt + p / kKvPage], j = p % kKvPage;
+  if (id < 0 || id >= a.s.pages || h >= a.H) return;
+  uint8_t *blk = a.base + ((int64_t)id * a.H + h) * kv_block_bytes(KIND, D);
+  const f32x8 k = load8<TYPE>(a.k, row, h * D + part * 8), v = load8<TYPE>(a.v, row, h * D + part * 8);
+  if constexpr (KIND == kKvI8) {
+    uint32_t mk = 0, mv = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      mk = max(mk, __float_as_uint(k[i]) & 0x7FFFFFFFu);
+      mv = max(mv, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    }
+#pragma unroll
+    for (int x = 1; x < kParts; x <<= 1) {
+      mk = max(mk, (uint32_t)__shfl_xor((int)mk, x));
+      mv = max(mv, (uint32_t)__shfl_xor((int)mv, x));
+    }
+    float ks, vs;
+    const u32x2 kq = quantise(k, mk, &ks), vq = quantise(v, mv, &vs);
+    *(u32x2 *)(blk + kv_key_at(KIND, D, j, part * 8)) = kq;
+    if (part == 0) {
+      *(float *)(blk + kv_step_at(D, 0, j)) = ks;
+      *(float *)(blk + kv_step_at(D, 1, j)) = vs;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) blk[kv_value_at(KIND, D, j, part * 8 + i)] = (uint8_t)(vq[i >> 2] >> 8 * (i & 3));
+  } else {
+    *(u32x4 *)(blk + kv_key_at(KIND, D, j, part * 8)) = KIND == kKvBf16 ? to_bf16x8(k) : to_f16x8(k);
+    const u32x4 vq = KIND == kKvBf16 ? to_bf16x8(v) : to_f16x8(v);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      *(uint16_t *)(blk + kv_value_at(KIND, D, j, part * 8 + i)) = (uint16_t)(vq[i >> 1] >> 16 * (i & 1));
   }
 }
 
@@ -297,10 +355,17 @@ void each(F &&f) {  // every instance: cache kind, dim, row type
 }
 void launch(const KvArgs &a, bool write, hipStream_t s) {
   const dim3 grid((unsigned)kv_max_pieces(a.s.n, a.s.R, a.s.rows != nullptr), (unsigned)a.H);
+  // Few rows of a sequence: by rows, as a piece's workgroup of 64 tokens would idle; many: by pieces, whose stores are whole
+  // granules. Row kernel / piece kernel with 256 sequences, 8 heads of 128, us: 16 bits, 1 row each 5.2 / 12.6, 8 rows 14 / 19,
+  // 16 rows 33 / 21; 8 bits, 1 row 6.0 / 29, 32 rows 47 / 54, 64 rows 88 / 102; 32 sequences of 64 rows, 8 bits: 15 / 13.
+  const bool few = a.s.R <= (a.kind == kKvI8 ? 32 : 8) * (int64_t)a.s.n;
   each([&](auto kind, auto dim, auto type) {
     constexpr int K = decltype(kind)::value, D = decltype(dim)::value, T = decltype(type)::value;
     if (a.kind != K || a.D != D || a.type != T) return;
-    if (write) hipLaunchKernelGGL((kv_write<K, D, T>), grid, dim3(kThreads<D>), 0, s, a);
+    constexpr int kHeads = 512 / D;  // of a wave in kv_write_rows
+    if (write && few)
+      hipLaunchKernelGGL((kv_write_rows<K, D, T>), dim3((a.s.R + 3) / 4, (a.H + kHeads - 1) / kHeads), dim3(256), 0, s, a);
+    else if (write) hipLaunchKernelGGL((kv_write<K, D, T>), grid, dim3(kThreads<D>), 0, s, a);
     else hipLaunchKernelGGL((kv_read<K, D, T>), grid, dim3(kThreads<D>), 0, s, a);
   });
   IJ_HIP(hipGetLastError());

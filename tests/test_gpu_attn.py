@@ -139,6 +139,50 @@ def test_write_then_read(eng, cache, dtype, heads, dim):
             assert np.array_equal(got, cast(x, dtype)[1]), (layer, np.abs(got - x).max())
 
 
+@pytest.mark.parametrize("cache", ["BF16", "F16", "I8"])
+@pytest.mark.parametrize("dtype", ["F32", "BF16", "F16"])
+@pytest.mark.parametrize("heads,dim", [(1, 64), (9, 64), (5, 128), (2, 256), (3, 256)])
+def test_few_rows_of_each_sequence(eng, cache, dtype, heads, dim):
+    """no row to five of each sequence, between rows of none, some before token 0, in no page, not finite: the same bytes as
+    whole sequences written"""
+    print(cache, dtype, heads, dim, flush=True)
+    rng = np.random.default_rng(7 * dim + heads)
+    lens = [1, 63, 64, 66, 200, 0, 3, 130, 65]
+    new = [1, 0, 3, 4, 2, 0, 5, 1, 5]
+    pool = Pool(rng, lens)
+    table = pool.table.copy()
+    table[8, 1] = pool.pages  # the last sequence's token 64
+    T, lead = sum(lens), 2
+    k, v = rows_like(rng, T, heads, dim), rows_like(rng, T, heads, dim)
+    at = offsets(lens)
+    k[at[4] - 1, 0, 3], v[at[4] - 2, heads - 1, dim - 1], k[at[3] - 1] = np.inf, np.nan, 0
+    (kr, kv_), (vr, vv_) = cast(k, dtype), cast(v, dtype)
+    few, full = (eng.kv_create(1, pool.pages, heads, dim, cache) for _ in range(2))
+    whole = batch(eng, pool.table, lens, at)
+    full.write_bufs(0, whole, T, up(eng, kr), up(eng, vr), dtype)
+    few.write_bufs(0, whole, T, up(eng, np.zeros_like(kr)), up(eng, np.zeros_like(vr)), dtype)
+    src, mine = [], []
+    for b, m in enumerate(new):
+        for i in range(m):
+            t = lens[b] - m + i
+            src.append(at[b] + t if t >= 0 else 0)
+            if t >= 0 and not (b == 8 and t == 64):
+                mine.append(at[b] + t)
+    R = lead + len(src) + 3
+    rows_k, rows_v = np.full((R, heads, dim), 9, kr.dtype), np.full((R, heads, dim), 9, vr.dtype)
+    rows_k[lead:lead + len(src)], rows_v[lead:lead + len(src)] = kr[src], vr[src]
+    few.write_bufs(0, batch(eng, table, lens, offsets(new) + np.int32(lead)), R, up(eng, rows_k), up(eng, rows_v), dtype)
+    got = []
+    for c in (full, few):
+        bufs = [eng.alloc(T * heads * dim * 4) for _ in range(2)]
+        c.read_bufs(0, whole, T, *bufs)
+        got.append([b.download(np.uint32, (T, heads, dim)) for b in bufs])
+    for a, b in zip(*got):
+        want = np.zeros_like(a)
+        want[mine] = a[mine]
+        assert np.array_equal(b, want)
+
+
 @pytest.mark.parametrize("cache", ["BF16", "I8"])
 def test_cache_strides_offsets_and_single_rows(eng, cache):
     """rows inside wider rows (q, k, v side by side), at an offset, one per sequence without a row table; rows that no
