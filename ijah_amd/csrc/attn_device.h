@@ -28,28 +28,43 @@ __device__ __forceinline__ const void *again(const void *p) {  // the same of a 
 // (the type is a template argument: with a run-time one, the compiler dropped the fp16 branch of a copy whose two conversions
 // cancel)
 template <int TYPE>
-__device__ __forceinline__ f32x8 load8(const RowMat &m, int64_t row, int col) {
+struct Raw8 {
+  u32x4 w[TYPE == kRowF32 ? 2 : 1];
+};
+template <int TYPE>
+__device__ __forceinline__ Raw8<TYPE> load_raw8(const RowMat &m, int64_t row, int col) {
   const int64_t i = row * m.ld + col;
+  Raw8<TYPE> r;
+  if constexpr (TYPE == kRowF32) {
+    r.w[0] = *(const u32x4 *)((const float *)m.p + i);
+    r.w[1] = *(const u32x4 *)((const float *)m.p + i + 4);
+  } else {
+    r.w[0] = *(const u32x4 *)((const uint16_t *)m.p + i);
+  }
+  return r;
+}
+template <int TYPE>
+__device__ __forceinline__ f32x8 widen8(const Raw8<TYPE> &r) {
   f32x8 o;
   if constexpr (TYPE == kRowF32) {
-    const f32x4 a = *(const f32x4 *)((const float *)m.p + i), b = *(const f32x4 *)((const float *)m.p + i + 4);
 #pragma unroll
-    for (int k = 0; k < 4; k++) o[k] = a[k], o[4 + k] = b[k];
-  } else {
-    const u32x4 w = *(const u32x4 *)((const uint16_t *)m.p + i);
-    if constexpr (TYPE == kRowBf16) {
+    for (int k = 0; k < 8; k++) o[k] = __uint_as_float(r.w[k >> 2][k & 3]);
+  } else if constexpr (TYPE == kRowBf16) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        o[2 * k] = __uint_as_float(w[k] << 16);
-        o[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-      }
-    } else {
-      const f16x8 h = __builtin_bit_cast(f16x8, w);
-#pragma unroll
-      for (int k = 0; k < 8; k++) o[k] = (float)h[k];
+    for (int k = 0; k < 4; k++) {
+      o[2 * k] = __uint_as_float(r.w[0][k] << 16);
+      o[2 * k + 1] = __uint_as_float(r.w[0][k] & 0xFFFF0000u);
     }
+  } else {
+    const f16x8 h = __builtin_bit_cast(f16x8, r.w[0]);
+#pragma unroll
+    for (int k = 0; k < 8; k++) o[k] = (float)h[k];
   }
   return o;
+}
+template <int TYPE>
+__device__ __forceinline__ f32x8 load8(const RowMat &m, int64_t row, int col) {
+  return widen8<TYPE>(load_raw8<TYPE>(m, row, col));
 }
 __device__ __forceinline__ u32x4 to_bf16x8(const f32x8 &v) {
   bf16x8 o;

@@ -2,13 +2,15 @@
 //
 // Write: 16 bits c = round(x); 8 bits s = max|x| f32(1 / 127) over the head's dims, c = clamp(round(x / s)). Both are copies with
 // a change of layout, bound by HBM when there is enough to move and by the launch and three dependent loads (lengths,
-// page id, rows) otherwise.
+// page id, rows) otherwise. 16 sequences of 4096 tokens, 8 heads of 128, bf16 rows: write 110 us (4.9 TB/s) into 16 bits, 89 us
+// (4.5 TB/s) into 8; read 107 us (5.0 TB/s) and 92 us (4.4 TB/s). A large copy reaches 5.1 TB/s.
 //
-// A workgroup takes one piece (the rows of one sequence that lie in one page) of one key head, so that no two write into
-// one 16-byte granule of the values. Thread (token t % 16, part t / 16) holds 8 dims of a token: a wave then reads 16
-// rows x 32 dims, and its keys are 64 consecutive granules, 1 KB a store. Values go through LDS once: rows of the tile in,
-// 8 keys of one dim out. A granule whose 8 keys all are the piece's is one store; at a piece's ends the values of its
-// keys are stored alone, the other bytes belong to other tokens.
+// Many rows: a workgroup takes one piece (the rows of one sequence that lie in one page) of one key head, so that no two
+// write into one 16-byte granule of the values. Thread (token t % 16, part t / 16) holds 8 dims of a token: a wave then
+// reads 16 rows x 32 dims, and its keys are 64 consecutive granules, 1 KB a store. The rows are held as they were loaded until
+// their turn: widened they took 172 registers with 8 bits, two waves a SIMD, and 177 us for the write above. Values go
+// through LDS once: rows of the tile in, 8 keys of one dim out. A granule whose 8 keys all are the piece's is one store; at a
+// piece's ends the values of its keys are stored alone, the other bytes belong to other tokens.
 #include "attn_device.h"
 #include "common.h"
 
@@ -57,16 +59,31 @@ __device__ __forceinline__ bool find_piece(const KvSeqs &s, int item, int *sum, 
   return true;
 }
 
-// 8 of a row's elements in steps of its largest magnitude (as bits: an infinity or a NaN is larger than any number) / 127
+// 8 of a row's elements in steps of its largest magnitude (as bits: an infinity or a NaN is larger than any number) / 127.
+// x times the step's reciprocal is within 127 (2^-24 + 2^-24) < 2^-15 of the f32 quotient, so both round to the same integer
+// unless the product lies within 2^-14 of a half (1 element in 8192) or the reciprocal overflows: then the quotient itself.
 __device__ __forceinline__ u32x2 quantise(const f32x8 &x, uint32_t m, float *step) {
+  constexpr float kInt = 0x1.8p23f;  // added: a product rounded to an integer, which is the sum's low bits
   const float s = m < 0x7F800000u ? __uint_as_float(m) * (1.f / 127.f) : __builtin_nanf("");
   *step = s;
-  u32x2 o = {0u, 0u};
+  const float inv = 1.f / s;
+  uint32_t q[8];
+  float far = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float c = s > 0.f ? fminf(fmaxf(rintf(x[i] / s), -127.f), 127.f) : 0.f;
-    o[i >> 2] |= ((uint32_t)(int)c & 0xFFu) << (8 * (i & 3));
+    const float f = __builtin_fmaf(x[i], inv, kInt);
+    far = fmaxf(far, fabsf(__builtin_fmaf(x[i], inv, -(f - kInt))));
+    q[i] = __float_as_uint(f);
   }
+  if (far > 0.5f - 0x1p-14f || !(inv < 0x1p126f)) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = (uint32_t)(int)(s > 0.f ? fminf(fmaxf(rintf(x[i] / s), -127.f), 127.f) : 0.f);
+  }
+  u32x2 o;
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+    o[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[4 * i + 3], q[4 * i + 2], 0x0C0C0400u),
+                                 __builtin_amdgcn_perm(q[4 * i + 1], q[4 * i], 0x0C0C0400u), 0x05040100u);
   return o;
 }
 
@@ -81,16 +98,13 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
   if (!find_piece<NT>(a.s, (int)blockIdx.x, sum, &p) || p.page < 0) return;
   uint8_t *blk = a.base + ((int64_t)p.page * a.H + h) * kv_block_bytes(KIND, D);
   // all of the piece's rows are requested at once: four groups of 16 tokens
-  f32x8 k[4], v[4];
+  Raw8<TYPE> kr[4] = {}, vr[4] = {};
 #pragma unroll
   for (int g = 0; g < 4; g++) {
     const int j = g * 16 + tok;
     if (j >= p.j0 && j < p.j1) {
-      k[g] = load8<TYPE>(a.k, p.row0 + j - p.j0, h * D + part * 8);
-      v[g] = load8<TYPE>(a.v, p.row0 + j - p.j0, h * D + part * 8);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++) k[g][i] = v[g][i] = 0.f;
+      kr[g] = load_raw8<TYPE>(a.k, p.row0 + j - p.j0, h * D + part * 8);
+      vr[g] = load_raw8<TYPE>(a.v, p.row0 + j - p.j0, h * D + part * 8);
     }
   }
   if constexpr (KIND == kKvI8) {
@@ -98,10 +112,11 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
 #pragma unroll
     for (int g = 0; g < 4; g++) {
       uint32_t mk = 0, mv = 0;
+      const f32x8 k = widen8<TYPE>(kr[g]), v = widen8<TYPE>(vr[g]);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        mk = max(mk, __float_as_uint(k[g][i]) & 0x7FFFFFFFu);
-        mv = max(mv, __float_as_uint(v[g][i]) & 0x7FFFFFFFu);
+        mk = max(mk, __float_as_uint(k[i]) & 0x7FFFFFFFu);
+        mv = max(mv, __float_as_uint(v[i]) & 0x7FFFFFFFu);
       }
 #pragma unroll
       for (int x = 16; x < 64; x <<= 1) {
@@ -119,6 +134,7 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
   for (int g = 0; g < 4; g++) {
     const int j = g * 16 + tok;
     const bool on = j >= p.j0 && j < p.j1;
+    const f32x8 k = widen8<TYPE>(kr[g]), v = widen8<TYPE>(vr[g]);
     if constexpr (KIND == kKvI8) {
       uint32_t mk = 0, mv = 0;
 #pragma unroll
@@ -128,7 +144,7 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
       }
       if (on) {
         float ks, vs;
-        const u32x2 kq = quantise(k[g], mk, &ks), vq = quantise(v[g], mv, &vs);
+        const u32x2 kq = quantise(k, mk, &ks), vq = quantise(v, mv, &vs);
         *(u32x2 *)(blk + kv_key_at(KIND, D, j, part * 8)) = kq;
         if (part == 0) {
           *(float *)(blk + kv_step_at(D, 0, j)) = ks;
@@ -139,8 +155,8 @@ __global__ __launch_bounds__(kThreads<D>) void kv_write(KvArgs a) {
         t[1] = vq[1];
       }
     } else if (on) {
-      *(u32x4 *)(blk + kv_key_at(KIND, D, j, part * 8)) = KIND == kKvBf16 ? to_bf16x8(k[g]) : to_f16x8(k[g]);
-      const u32x4 vq = KIND == kKvBf16 ? to_bf16x8(v[g]) : to_f16x8(v[g]);
+      *(u32x4 *)(blk + kv_key_at(KIND, D, j, part * 8)) = KIND == kKvBf16 ? to_bf16x8(k) : to_f16x8(k);
+      const u32x4 vq = KIND == kKvBf16 ? to_bf16x8(v) : to_f16x8(v);
       word *t = (word *)(tile + j * kPitch + part * 16);
 #pragma unroll
       for (int i = 0; i < 4; i++) t[i] = vq[i];
@@ -356,9 +372,9 @@ void each(F &&f) {  // every instance: cache kind, dim, row type
 void launch(const KvArgs &a, bool write, hipStream_t s) {
   const dim3 grid((unsigned)kv_max_pieces(a.s.n, a.s.R, a.s.rows != nullptr), (unsigned)a.H);
   // Few rows of a sequence: by rows, as a piece's workgroup of 64 tokens would idle; many: by pieces, whose stores are whole
-  // granules. Row kernel / piece kernel with 256 sequences, 8 heads of 128, us: 16 bits, 1 row each 5.2 / 12.6, 8 rows 14 / 19,
-  // 16 rows 33 / 21; 8 bits, 1 row 6.0 / 29, 32 rows 47 / 54, 64 rows 88 / 102; 32 sequences of 64 rows, 8 bits: 15 / 13.
-  const bool few = a.s.R <= (a.kind == kKvI8 ? 32 : 8) * (int64_t)a.s.n;
+  // granules. Row kernel / piece kernel with 256 sequences, 8 heads of 128, us: 16 bits, 1 row each 5.2 / 11.1, 8 rows 14 / 18,
+  // 16 rows 34 / 21, 64 rows 88 / 39; 8 bits 5.7 / 15.5, 15 / 22, 26 / 25, 86 / 52.
+  const bool few = a.s.R <= 12 * (int64_t)a.s.n;
   each([&](auto kind, auto dim, auto type) {
     constexpr int K = decltype(kind)::value, D = decltype(dim)::value, T = decltype(type)::value;
     if (a.kind != K || a.D != D || a.type != T) return;

@@ -183,6 +183,30 @@ def test_few_rows_of_each_sequence(eng, cache, dtype, heads, dim):
         assert np.array_equal(b, want)
 
 
+@pytest.mark.parametrize("rows", [12, 700])
+def test_eight_bit_values_around_halves(eng, rows):
+    """quotients at a half and within a few ulp of one, rows of every magnitude down to the smallest subnormals: as the plain
+    form's division and rounding say"""
+    rng = np.random.default_rng(rows)
+    dim = 64
+    top = np.ldexp(np.float32(1), rng.integers(-149, 127, rows)).astype(np.float32) * rng.uniform(1, 2, rows).astype(np.float32)
+    top[:4] = [2.0 ** -149, 2.0 ** -126, 3.4e38, 127]
+    step = top * (np.float32(1) / np.float32(127))
+    x = (step[:, None] * (rng.integers(-127, 127, (rows, dim)) + 0.5).astype(np.float32)).astype(np.float32)
+    for i in range(dim):  # up to three ulp off
+        for _ in range(i % 4):
+            x[:, i] = np.nextafter(x[:, i], np.float32(np.inf if i & 4 else 0))
+    x = np.clip(x, -top[:, None], top[:, None])
+    x[:, 5] = top
+    pool = Pool(rng, [rows])
+    kv = eng.kv_create(1, pool.pages, 1, dim, "I8")
+    seqs = batch(eng, pool.table, [rows], offsets([rows]))
+    kv.write(0, seqs, x, -x)
+    k, v = kv.read(0, seqs, rows)
+    want = held(x, "I8")
+    assert np.array_equal(k.reshape(rows, dim), want) and np.array_equal(v.reshape(rows, dim), -want)
+
+
 @pytest.mark.parametrize("cache", ["BF16", "I8"])
 def test_cache_strides_offsets_and_single_rows(eng, cache):
     """rows inside wider rows (q, k, v side by side), at an offset, one per sequence without a row table; rows that no
