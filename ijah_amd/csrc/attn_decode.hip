@@ -16,10 +16,18 @@
 // weights' factors, are taken relative to the largest power of two that the wave has met (taken back at the end). What a
 // part then drops is 2^-24 of the largest element or weight at most.
 //
-// Work is dealt out in equal shares of pages over one workgroup per CU, so a single long sequence and a ragged batch fill
-// the chip alike; a workgroup's waves take a segment's pages in turn and are joined through LDS, shares of one group
-// through its partials, by the last of them to arrive (a counter; partials are device-coherent stores, so no cache is
-// written back or invalidated).
+// Work is dealt out in units of a page over as many workgroups as the chip holds (two a CU, one with 256 dims), so a single
+// long sequence and a ragged batch fill it alike: one chunk of a group for each workgroup where the groups fit them, else equal
+// shares; the device does it, so a captured call follows the lengths. A workgroup's waves take a segment's pages in turn and
+// are joined through LDS, the parts of one group through memory by the last of them to arrive (a counter; partials are
+// device-coherent stores, so no cache is written back or invalidated). Many rows (drafts, or more than 16 query heads to a
+// key head) go in blocks of 32, two blocks of a group side by side so that their reads of a page meet in the caches, and
+// their parts are joined by a launch of their own.
+//
+// Measured: one sequence of 131072 tokens, 2 key heads of 256, bf16: 64 us for 268 MB (4.2 TB/s; a large copy reaches 5.1). 48
+// ragged sequences of up to 4000 tokens, 4 key heads of 128, 8 bits: 24 us for 70 MB. One of 37 tokens: 7.5 us, of which the
+// call's host side is 5. Sixteen sequences of up to 16000 tokens with up to six drafts of 80 heads over 5 of 128: 76 us for
+// 203 MB and 38 GFLOP of part products (40 and 30 us), as products and exponentials of one SIMD overlap little.
 #include "attn_device.h"
 #include "common.h"
 

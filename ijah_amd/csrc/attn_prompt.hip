@@ -13,6 +13,11 @@
 // 32-bit rows are cut into NT = 3 bf16 parts (8 bits each) and each product is the sum of the six part products that
 // reach 2^-24: exact to f32's own rounding at six times the matrix work, with f32's range. 16-bit rows are products of
 // their own type (NT = 1), the weights rounded to it (2^-9 or 2^-12 of each, as the output itself); sums are f32.
+//
+// Measured: fp16, 2048 rows over 16048 keys, 16 heads over 2 of 256: 539 us, 935 TFLOP/s (a library product of 8192^3 reaches
+// 1213); the matrix cores are busy for 44% of their SIMDs' cycles and the vector ALUs for 42%, mostly one after the other.
+// Nine packed sequences of 3231 tokens, bf16, 32 heads over 4 of 128: 38 us, the longest one's last blocks. 32 bits, 4096
+// tokens, 64 heads over 8 of 64: 722 us, 1142 TFLOP/s of part products.
 #include "attn_device.h"
 #include "common.h"
 

@@ -37,8 +37,8 @@ NE_API void ne_kv_free(ne_kv *kv);
 NE_API int ne_kv_info(const ne_kv *kv, ne_kv_desc *d, uint64_t *bytes);
 
 /* A batch of sequences. Sequence b has lens[b] tokens in the cache after this step; token p is in page table[b][p / 64]
- * at p % 64. rows: i32 [n + 1]; rows[b] .. rows[b + 1] - 1 are the call's rows of sequence b, its newest tokens: the
- * last of them is token lens[b] - 1 (NULL: one row each, row b). All three live on the device and are read by the
+ * at p % 64. rows: i32 [n + 1], ascending; rows[b] .. rows[b + 1] - 1 are the call's rows of sequence b, its newest tokens:
+ * the last of them is token lens[b] - 1 (NULL: one row each, row b). All three live on the device and are read by the
  * kernels, so a captured call takes what they hold at the replay. What they hold is bounds-checked there: a length
  * outside 0 .. 64 ldt and rows outside 0 .. R are clamped, a page id outside the handle's pages is a page without
  * tokens (not written, read as zeros, not attended), and a row before token 0 is not written, is zero when read, and
@@ -57,20 +57,21 @@ NE_API int ne_kv_read(const ne_kv *kv, int layer, const ne_kv_seqs *s, int R, ne
 /* Attention of the R newest tokens over the cache, which holds them already: for the row of token p, query head h (of
  * `heads`, a multiple of the handle's; key head h / (heads / handle's heads)): out = sum_{j <= p} softmax_j(scale q .
  * k_j) v_j. A row that sees no token is zero. out has q's type; it may be q's own rows. One launch for any mixture of
- * lengths; results of one call do not vary from run to run (the sums' order follows the batch's lengths). What a row does
- * not see may hold anything, infinities and NaN included; a row that sees a key or a value that is not finite is not finite
- * where that enters it. n tables of ldt pages and R rows of `heads` heads must stay below 2^31 units of work (a page for 16
- * rows of a key head), all counted as full: larger batches are refused. */
+ * lengths (and one that joins the parts of long sequences, where there are more rows than sequences or more than 16 query
+ * heads to a key head); results of one call do not vary from run to run (the sums' order follows the batch's lengths).
+ * What a row does not see may hold anything, infinities and NaN included; a row that sees a key or a value that is not
+ * finite is not finite where that enters it. n tables of ldt pages and R rows of `heads` heads must stay below 2^31 units
+ * of work (a page for 16 rows of a key head), all counted as full: larger batches are refused. */
 NE_API int ne_attn_decode(ne_kv *kv, int layer, const ne_kv_seqs *s, int R, int heads, const ne_buf *q, uint64_t q_off,
                           int ldq, ne_buf *out, uint64_t out_off, int ldo, int dtype, float scale, double *gpu_ms);
 
 /* ---- packed prompts ----
- * n sequences packed behind one another: rows q_rows[b] .. q_rows[b + 1] - 1 of q and out, rows k_rows[b] .. k_rows[b + 1]
- * - 1 of k and v (i32 [n + 1] on the device; k_rows NULL: q_rows; values outside 0 .. Rq / Rk are clamped). Causal with the
- * ends aligned: row i of nq sees the keys j <= i + nk - nq; one that sees none is zero. Query head h uses key head h /
- * (heads / kv_heads). Rows of out that no sequence names are left as they were; out may not overlap q, k or v. Masked keys and
- * values may hold anything, as above. 16-bit rows: products of that type summed in f32, the softmax weights rounded to it.
- * 32-bit rows: products exact to f32's rounding. */
+ * n sequences packed behind one another: rows q_rows[b] .. q_rows[b + 1] - 1 of q and out, rows k_rows[b] .. k_rows[b +
+ * 1] - 1 of k and v (i32 [n + 1], ascending, on the device; k_rows NULL: q_rows; values outside 0 .. Rq / Rk are
+ * clamped). Causal with the ends aligned: row i of nq sees the keys j <= i + nk - nq; one that sees none is zero. Query
+ * head h uses key head h / (heads / kv_heads). Rows of out that no sequence names are left as they were; out may not
+ * overlap q, k or v. Masked keys and values may hold anything, as above. 16-bit rows: products of that type summed in
+ * f32, the softmax weights rounded to it. 32-bit rows: products exact to f32's rounding. */
 typedef struct ne_attn_prompt_desc {
   int n, heads, kv_heads, dim, dtype; /* dtype of q, k, v and out: NE_F32, NE_BF16 or NE_F16 */
   int Rq, Rk;                         /* rows of q and out; of k and v */

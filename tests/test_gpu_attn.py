@@ -705,6 +705,56 @@ def test_two_graphs_of_one_cache(eng):
         hip.hipGraphDestroy(g)
 
 
+def test_captured_drafts(eng):
+    """a captured decode of drafts, whose parts a second launch joins: replays follow lengths and rows from long sequences to
+    one page, none and back, and leave what no sequence names"""
+    hip = hip_runtime()
+    rng = np.random.default_rng(43)
+    H, Hq, D, R = 2, 16, 128, 8
+    full = [9000, 700]
+    pool = Pool(rng, full)
+    kv = eng.kv_create(1, pool.pages, H, D, "F16")
+    k, v = rows_like(rng, sum(full), H, D), rows_like(rng, sum(full), H, D)
+    kv.write(0, batch(eng, pool.table, full, offsets(full)), k, v)
+    kh, vh = held(k, "F16"), held(v, "F16")
+    q = rows_like(rng, R, Hq, D)
+    qb, ob = up(eng, q), up(eng, np.full((R, Hq, D), -99, np.float32))
+    seqs = batch(eng, pool.table, full, offsets([4, 4]))
+    eng.sync()
+    s, g, ex = eng.lib.ne_stream(), C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(s, 1) == 0
+    try:
+        kv.attend_bufs(0, seqs, R, Hq, qb, ob)
+    finally:
+        assert hip.hipStreamEndCapture(s, C.byref(g)) == 0
+    try:
+        assert hip.hipGraphInstantiate(C.byref(ex), g, None, None, 0) == 0
+        for lens, new in (([9000, 700], [4, 4]), ([60, 3], [5, 3]), ([0, 700], [0, 8]), ([8999, 1], [7, 1]), ([5000, 0], [1, 0]),
+                          ([9000, 700], [4, 4])):
+            seqs.lens.upload(np.array(lens, np.int32))
+            seqs.rows.upload(offsets(new))
+            ob.upload(np.full((R, Hq, D), -99, np.float32))
+            assert hip.hipGraphLaunch(ex, s) == 0
+            assert hip.hipStreamSynchronize(s) == 0
+            got = ob.download(np.float32, (R, Hq, D))
+            at = 0
+            for b, m in enumerate(new):
+                if m:
+                    o = b * full[0]
+                    last = [lens[b] - m + i for i in range(m)]
+                    check(got[at:at + m], plain(q[at:at + m], kh[o:o + lens[b]], vh[o:o + lens[b]], last, D ** -0.5), lens[b], D,
+                          "F32", False, (lens, new, b))
+                at += m
+            assert (got[at:] == -99).all()
+            eager = up(eng, np.full((R, Hq, D), -99, np.float32))
+            kv.attend_bufs(0, seqs, R, Hq, qb, eager)
+            assert np.array_equal(eager.download(np.float32, (R, Hq, D)), got)
+    finally:
+        if ex.value:
+            hip.hipGraphExecDestroy(ex)
+        hip.hipGraphDestroy(g)
+
+
 # ---------------------------------------------------------------------------------------------------- together
 def test_block_of_a_model(eng):
     """the trunk's q, k, v in one launch, the cache, decode and the o linear, step by step after a prompt: decode gives what
